@@ -143,7 +143,7 @@ def prepare(case, seed) -> dict:
     w = s.pop("w")
     if own:
         s["ops"] = _ops()
-        s["w"] = s["ops"].prepare_weight_mx4(w)
+        s["w"] = s["ops"].prepare_weight_mx4(w, gate_up=kind == "glu" or case.get("unit") == "gated")
     else:
         s["w"] = (*_quantized(w), w.shape[-1])
     del w
