@@ -109,6 +109,48 @@ class SplitParts:
         return self.float().to(dtype)
 
 
+class Mx4:
+    """Matrices ``[..., rows, K]`` held as 4-bit microscaled floating point (made by ``Ops.quantize_mx4`` or
+    ``Ops.prepare_weight_mx4``, read by the ``*_mx4`` products).
+
+    A row is cut into blocks of 32 values; a block has one scale, a power of two whose biased exponent is one byte
+    (255: the block is no number), and 32 codes of a sign, two exponent bits and one mantissa bit that stand for 0,
+    0.5, 1, 1.5, 2, 3, 4, 6.  ``codes``: uint8 ``[all rows, bytes]``, two codes a byte, the even place in the low bits;
+    ``scales``: uint8 ``[tiles, atoms, 512]`` in the order in which they enter the tensor cores (csrc/mx4.h)."""
+
+    __slots__ = ("codes", "scales", "shape", "gate_up")
+    TILE_ROWS = 128
+
+    def __init__(self, shape, device, gate_up: bool = False):
+        """Memory for matrices of this shape; ``gate_up``: pairs ``[..., 2, N, K]`` of a gate and an up matrix whose
+        rows lie interleaved, 16 and 16."""
+        self.shape, self.gate_up = tuple(int(n) for n in shape), bool(gate_up)
+        *lead, n, k = self.shape
+        mats = 1
+        for i in lead:
+            mats *= i
+        if gate_up:
+            mats, n = mats // 2, -(-n // 16) * 32
+        # (what fills up a pair's rows is read, so it is zeroed)
+        new = torch.empty if n == self.shape[-2] or n == 2 * self.shape[-2] else torch.zeros
+        self.codes = new((mats * n, self.pitch(k)), dtype=torch.uint8, device=device)
+        self.scales = new((mats * -(-n // self.TILE_ROWS), -(-k // 256) * 2, 512), dtype=torch.uint8, device=device)
+
+    @staticmethod
+    def pitch(k: int) -> int:
+        """Bytes of codes a row."""
+        return -(-k // 32) * 16
+
+    @staticmethod
+    def tile_bytes(k: int) -> int:
+        """Bytes of scales of 128 rows."""
+        return -(-k // 256) * 1024
+
+    @property
+    def device(self):
+        return self.codes.device
+
+
 class Ops:
     """The kernels, bound to one device.  Fails at construction without a GPU."""
 
@@ -915,6 +957,15 @@ class Ops:
                    "combine": _decl(lib, "mls_expert_combine",
                                     [_P, _I, _P, _I, _I, _LL, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I,
                                      _P])}
+        elif name == "mx4":
+            fns = {"quantize": _decl(lib, "mls_mx4_quantize",
+                                     [_P, _I, _LL, _LL, _I, _I, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P]),
+                   "values": _decl(lib, "mls_mx4_values", [_P, _P, _LL, _I, _I, _I, _P, _I, _P]),
+                   "product": _decl(lib, "mls_mx4_product",
+                                    [_I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _F, _P, _P]),
+                   "expert_product": _decl(lib, "mls_mx4_expert_product",
+                                           [_I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _I,
+                                            _F, _F, _P, _P])}
         elif name == "shortconv":
             fns = {"qk": _decl(lib, "mls_qk_conv_norm_rope_store",
                                [_P, _I, _LL, _P, _P, _I, _P, _P, _I, _F, _P, _LL, _I, _P, _P, _P, _P,
@@ -1380,6 +1431,174 @@ class Ops:
             _ptr(delta), _code(delta.dtype), t, d, self._stream()), "expert_combine")
         if isinstance(shared, SplitParts):
             shared.release()
+
+    # ------------------------------------------------- 4-bit microscaled rows and weights
+    def _mx4_source(self, x, what: str):
+        """(rows, K, row stride) of a matrix to be quantised."""
+        _need(isinstance(x, torch.Tensor) and x.dim() >= 2 and x.dtype in (torch.float32, torch.bfloat16),
+              f"{what}: rows [..., K] of float32 or bfloat16")
+        self._need_here(what, x)
+        k = x.shape[-1]
+        _need(1 <= k <= self.MX4_MOST_K, f"{what}: rows of 1 to {self.MX4_MOST_K} values, not {k}")
+        if x.dim() == 2:
+            _need(x.stride(1) == 1 or k == 1, f"{what}: a row's values must lie side by side")
+            _need(x.shape[0] <= 1 or x.stride(0) >= k, f"{what}: rows must not overlap")
+            return x.shape[0], k, max(x.stride(0), k)
+        _need(x.is_contiguous(), f"{what}: matrices must be contiguous")
+        return x.numel() // k, k, k
+
+    MX4_MOST_K = 1 << 20
+
+    def _need_here(self, what: str, *tensors) -> None:
+        for t in tensors:
+            _need(t is None or (t.device.type == "cuda" and t.device.index == self._device_index),
+                  f"{what}: tensors must be on {self.device}")
+
+    def quantize_mx4(self, x, into: Mx4 | None = None, gate_up: bool = False) -> Mx4:
+        """The rows of ``x [..., rows, K]`` (float32 or bfloat16; two-dimensional ones may have a row stride) as 4-bit
+        microscaled values.
+
+        A block of 32 with the largest magnitude m has the scale ``2^max(floor(log2 m) - 2, -127)``; a value becomes the
+        nearest of the eight magnitudes times the scale, on a tie the one with the even code, what is larger than 6 becomes
+        6.  A block that holds an infinity or a NaN is NaN as a whole.  The last block of a row is filled up with zeros.
+        ``into``: an ``Mx4`` of the same shape to be overwritten, instead of new memory.  ``gate_up``: ``x [..., 2, N, K]``
+        holds pairs of a gate and an up matrix, laid out for ``linear_glu_mx4`` and ``expert_glu_mx4``."""
+        rows, k, ld = self._mx4_source(x, "quantize_mx4")
+        _need(not gate_up or (x.dim() >= 3 and x.shape[-3] == 2), "quantize_mx4: gate_up goes with matrices [..., 2, N, K]")
+        if into is None:
+            into = Mx4(x.shape, x.device, gate_up)
+        _need(isinstance(into, Mx4) and into.shape == tuple(x.shape) and into.gate_up == bool(gate_up),
+              "quantize_mx4: into is laid out for something else")
+        self._need_here("quantize_mx4", into.codes)
+        self._quantize_mx4(x, ld, rows, k, x.shape[-2], into.codes, into.scales, pairs=gate_up)
+        return into
+
+    def _quantize_mx4(self, x, ld, rows, k, per_mat, codes, scales, work=None, top=1, n_experts=0, gather=False,
+                      pairs=False):
+        if rows == 0:
+            return
+        self.launches += 1
+        order, idx, offsets = (work["order"], work["idx"], work["offsets"]) if work is not None else (None,) * 3
+        _check(self._part_lib("mx4")["quantize"](
+            _ptr(x), _code(x.dtype), ld, rows, k, per_mat, 1 if pairs else 0, _ptr(order), _ptr(idx), _ptr(offsets), top, n_experts,
+            1 if gather else 0, _ptr(codes), _ptr(scales), self._stream()), "quantize_mx4")
+
+    def mx4_values(self, q: Mx4, out) -> None:
+        """What ``q`` stands for, into ``out`` (its shape, float32 or bfloat16; both hold it exactly)."""
+        _need(isinstance(q, Mx4), "mx4_values: codes and scales of quantize_mx4")
+        _need(tuple(out.shape) == q.shape and out.is_contiguous()
+              and out.dtype in (torch.float32, torch.bfloat16), "mx4_values: bad output")
+        self._need_here("mx4_values", q.codes, out)
+        if out.numel() == 0:
+            return
+        k = q.shape[-1]
+        self.launches += 1
+        _check(self._part_lib("mx4")["values"](_ptr(q.codes), _ptr(q.scales), out.numel() // k, k, q.shape[-2],
+                                               1 if q.gate_up else 0, _ptr(out), _code(out.dtype), self._stream()),
+               "mx4_values")
+
+    def prepare_weight_mx4(self, w, gate_up: bool = False) -> Mx4:
+        """A matrix ``[out, in]`` made ready for ``linear_mx4``, the experts' ``[E, out, in]``, or with ``gate_up`` the
+        pair ``[2, out, in]`` of gate and up for ``linear_glu_mx4`` and the experts' ``[E, 2, out, in]``."""
+        return self.quantize_mx4(w.contiguous(), gate_up=gate_up)
+
+    def _mx4_rows(self, a, m: int, k: int, what: str):
+        """Codes and scales of a product's rows: those of an ``Mx4``, or of a tensor quantised into scratch memory."""
+        if isinstance(a, Mx4):
+            self._need_here(what, a.codes)
+            return a.codes, a.scales
+        _, _, ld = self._mx4_source(a, what)
+        pitch, tiles = Mx4.pitch(k), -(-m // Mx4.TILE_ROWS)
+        held = self.scratch("mx4_rows", (m * pitch + tiles * Mx4.tile_bytes(k)) // 4 + 4).view(torch.uint8)
+        scales = held[:tiles * Mx4.tile_bytes(k)]
+        codes = held[scales.numel():]
+        self._quantize_mx4(a, ld, m, k, m, codes, scales)
+        return codes, scales
+
+    @staticmethod
+    def _mx4_weight(w, unit: int, lead: int, what: str) -> None:
+        gated = unit == 1
+        _need(isinstance(w, Mx4) and len(w.shape) == lead + 2 + gated and w.gate_up == gated,
+              f"{what}: the weight comes from prepare_weight_mx4{' with gate_up' if gated else ''}, "
+              f"{lead + 2 + gated} dimensions")
+
+    def _product_mx4(self, unit: int, a, w: Mx4, out, what: str, alpha=1.0, limit=0.0) -> None:
+        self._mx4_weight(w, unit, 0, what)
+        _need(len(a.shape) == 2 and out.dim() == 2, f"{what}: shapes do not fit")
+        m, k = a.shape
+        n = w.shape[-2]
+        _need(w.shape[-1] == k and out.shape == (m, n), f"{what}: shapes do not fit")
+        _need(out.dtype in (torch.float32, torch.bfloat16) and out.is_contiguous(), f"{what}: bad output")
+        self._need_here(what, w.codes, out)
+        if m == 0 or n == 0:
+            return
+        codes, scales = self._mx4_rows(a, m, k, what)
+        self.launches += 1
+        _check(self._part_lib("mx4")["product"](
+            unit, _ptr(codes), _ptr(scales), _ptr(w.codes), _ptr(w.scales), _ptr(out),
+            _code(out.dtype), m, n, k, float(alpha), float(limit), _ptr(self.status),
+            self._stream()), what)
+
+    def linear_mx4(self, a, w: Mx4, out) -> None:
+        """``out[M, N] = q(a) @ w^T`` with float32 accumulation: rows and weights in 4-bit microscaled values.
+        ``a [M, K]``: float32 or bfloat16 rows, quantised on the way, or an ``Mx4``; ``w``: ``prepare_weight_mx4`` of a
+        matrix ``[N, K]``; ``out``: float32 or bfloat16."""
+        self._product_mx4(0, a, w, out, "linear_mx4")
+
+    def linear_glu_mx4(self, a, w_gate_up: Mx4, out, alpha: float = 1.0, limit: float = 0.0) -> None:
+        """``out[M, N] = silu(q(a) Wg^T) * (q(a) Wu^T)`` in one kernel behind the rows' quantisation;
+        ``w_gate_up``: ``prepare_weight_mx4`` of ``[2, N, K]`` with ``gate_up``.  ``limit`` > 0: the clamped unit of
+        ``linear_clamped_glu`` instead."""
+        self._product_mx4(1, a, w_gate_up, out, "linear_glu_mx4", alpha, limit)
+
+    def linear_relu_squared_mx4(self, a, w: Mx4, out) -> None:
+        """``out[M, N] = relu(q(a) @ w^T)^2``."""
+        self._product_mx4(2, a, w, out, "linear_relu_squared_mx4")
+
+    def _expert_product_mx4(self, unit: int, rows, w: Mx4, out, work: dict, top: int, scale: bool, what: str,
+                            alpha=1.0, limit=0.0) -> None:
+        self._mx4_weight(w, unit, 1, what)
+        n_experts, n, k = w.shape[0], w.shape[-2], w.shape[-1]
+        slots = out.shape[0]
+        _need(out.dim() == 2 and out.shape[1] == n and out.is_contiguous() and top >= 1 and slots % top == 0
+              and out.dtype in ((torch.float32,) if unit == 0 else (torch.float32, torch.bfloat16)),
+              f"{what}: bad output")
+        source_rows, source_k, ld = self._mx4_source(rows, what)
+        _need(rows.dim() == 2 and source_k == k and source_rows == (slots if unit == 0 else slots // top),
+              f"{what}: rows do not fit")
+        for name, dtype, least in (("order", torch.int32, slots), ("idx", torch.int32, slots),
+                                   ("offsets", torch.int32, n_experts + 1), ("weight", torch.float32, slots)):
+            held = work[name]
+            _need(held.dtype == dtype and held.is_contiguous() and held.numel() >= least, f"{what}: bad routing ({name})")
+            self._need_here(what, held)
+        self._need_here(what, w.codes, out)
+        if slots == 0 or n_experts == 0 or n == 0:
+            return
+        pitch, tiles = Mx4.pitch(k), slots // Mx4.TILE_ROWS + n_experts + 1
+        held = self.scratch("mx4_rows", (slots * pitch + tiles * Mx4.tile_bytes(k)) // 4 + 4).view(torch.uint8)
+        scales = held[:tiles * Mx4.tile_bytes(k)]
+        codes = held[scales.numel():]
+        self._quantize_mx4(rows, ld, slots, k, slots, codes, scales, work, top, n_experts, unit != 0)
+        self.launches += -(-n_experts // 1024)
+        _check(self._part_lib("mx4")["expert_product"](
+            unit, _ptr(codes), _ptr(scales), _ptr(w.codes), _ptr(w.scales), _ptr(out),
+            _code(out.dtype), slots, n_experts, n, k, _ptr(work["order"]), _ptr(work["offsets"]),
+            _ptr(work["weight"]), 1 if scale else 0, float(alpha), float(limit), _ptr(self.status), self._stream()), what)
+
+    def expert_glu_mx4(self, h, w_gate_up: Mx4, y, work: dict, top: int, scale_in: bool,
+                       alpha: float = 1.0, limit: float = 0.0) -> None:
+        """``expert_glu`` with 4-bit microscaled rows and weights; ``w_gate_up``: ``prepare_weight_mx4`` of
+        ``[E, 2, F, K]`` with ``gate_up``.  With ``scale_in`` a slot's weight multiplies the two float32 sums (the rows are quantised
+        without it).  Rows of ``y`` behind the last expert's are left as they are."""
+        self._expert_product_mx4(1, h, w_gate_up, y, work, top, scale_in, "expert_glu_mx4", alpha, limit)
+
+    def expert_relu_squared_mx4(self, h, w_up: Mx4, y, work: dict, top: int, scale_in: bool) -> None:
+        """``expert_relu_squared`` in the same way; ``w_up``: of ``[E, F, K]``."""
+        self._expert_product_mx4(2, h, w_up, y, work, top, scale_in, "expert_relu_squared_mx4")
+
+    def expert_down_mx4(self, y, w_down: Mx4, per_slot, work: dict, top: int, scale_out: bool) -> None:
+        """``expert_down`` in the same way; ``w_down``: of ``[E, D, F]``, ``per_slot`` float32."""
+        self._expert_product_mx4(0, y, w_down, per_slot, work, top, scale_out, "expert_down_mx4")
 
     def add_tanh_norm(self, x, delta, norm, h, post=None, bias=None, rows=None, n_rows: int = 0,
                       y_out=None) -> None:

@@ -53,7 +53,12 @@ MODULES = {
     "side": ["side_input.cu"],
     "gatednorm": ["gated_norm.cu"],
     "delta": ["delta_rule.cu", "delta_chunk.cu"],
+    # 4-bit microscaled rows and weights: built when such a weight is prepared
+    "mx4": ["mx4.cu", "mx4_gemm.cu"],
 }
+
+# headers of other modules' sources that a module's sources include
+SHARED_HEADERS = {"mx4": ["experts.h"]}
 
 
 def all_modules(head_sizes=()) -> list:
@@ -66,7 +71,7 @@ def all_modules(head_sizes=()) -> list:
     out.append(("argmax_static", {}))
     out += [(name, {}) for name in ("layernorm", "tanhnorm", "latent", "mlstm", "experts",
                                     "shortconv", "scan", "headprep", "side", "gatednorm",
-                                    "delta")]
+                                    "delta", "mx4")]
     return out
 
 
@@ -113,7 +118,8 @@ def _build_dir() -> Path:
 def _module_key(name: str, defines: dict) -> tuple:
     sources = MODULES[name]
     h = hashlib.sha256()
-    own_headers = [CSRC / (Path(s).stem + ".h") for s in sources]
+    own_headers = ([CSRC / (Path(s).stem + ".h") for s in sources]
+                   + [CSRC / h for h in SHARED_HEADERS.get(name, ())])
     for f in (sorted(CSRC.glob("*.cuh")) + [h for h in own_headers if h.is_file()]
               + [CSRC / s for s in sources]):
         h.update(f.name.encode())

@@ -1,0 +1,220 @@
+"""4-bit microscaled rows and their products against 64 bits."""
+
+import pytest
+import torch
+
+import plain_mx4 as plain
+from mini_llm_stack_b200.ops.kernels import KernelError, Mx4, Runtime
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    return Runtime("cuda:0", torch.bfloat16).ops
+
+
+def gen(*key):
+    return torch.Generator().manual_seed(hash(key) % (1 << 31))
+
+
+def values(ops, q, dtype=torch.float32):
+    out = torch.full(q.shape, -5.0, dtype=dtype, device="cuda")
+    ops.mx4_values(q, out)
+    return out.cpu()
+
+
+def same(a, b):
+    return torch.equal(torch.nan_to_num(a.double(), nan=12345.0), torch.nan_to_num(b.double(), nan=12345.0))
+
+
+def wide_rows(rows, k, g):
+    """Rows whose blocks' sizes spread over many powers of two, with zeros and ties among them."""
+    x = torch.randn(rows, k, generator=g) * torch.exp2(torch.randint(-20, 20, (rows, k // 32 + 1), generator=g).float()
+                                                       ).repeat_interleave(32, 1)[:, :k]
+    x[torch.rand(rows, k, generator=g) < 0.1] = 0.0
+    ties = torch.randint(-32, 33, (rows, k), generator=g).float() / 4
+    return torch.where(torch.rand(rows, 1, generator=g) < 0.3, ties, x)
+
+
+SHAPES = [(1, 1), (1, 31), (2, 32), (3, 33), (5, 64), (7, 255), (128, 256), (129, 257), (130, 96), (300, 1000), (1, 14336)]
+
+
+@pytest.mark.parametrize("rows, k", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_become_the_nearest_values(ops, rows, k, dtype):
+    x = wide_rows(rows, k, gen(rows, k)).to(dtype)
+    q = ops.quantize_mx4(x.cuda())
+    assert q.shape == (rows, k)
+    want = plain.nearest(x)
+    for out in (torch.float32, torch.bfloat16):
+        assert same(values(ops, q, out), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_ends_of_the_range(ops, dtype):
+    info = torch.finfo(dtype)
+    sub = 2.0 ** -133 if dtype == torch.bfloat16 else 2.0 ** -149
+    rows = [[sub] * 32, [0.0] * 32, [-0.0] * 32, [info.max] * 32, [-info.max, sub] * 16, [2.0 ** -127 * 1.25, 2.0 ** -128] * 16,
+            [info.smallest_normal] * 32, [2.0 ** -124, 2.0 ** -127] * 16, [float("inf")] + [1.0] * 31,
+            [1.0] * 31 + [float("-inf")], [float("nan")] + [0.0] * 31, [1.0] * 31 + [float("nan")]]
+    x = torch.tensor(rows, dtype=torch.float64).to(dtype)
+    x = torch.cat([x, torch.ones(len(rows), 32, dtype=dtype)], 1)       # the block beside is a number
+    got = values(ops, ops.quantize_mx4(x.cuda()))
+    assert same(got, plain.nearest(x))
+    assert torch.equal(got[:, 32:], torch.ones(len(rows), 32))
+
+
+def test_rows_between_addresses_and_with_strides(ops):
+    g = gen("strides")
+    for dtype in (torch.bfloat16, torch.float32):
+        big = wide_rows(40, 500, g).to(dtype).cuda()
+        for view in (big[:, :256], big[:, 1:258], big[::2, 8:264], big[3:9, 100:133]):
+            assert same(values(ops, ops.quantize_mx4(view)), plain.nearest(view.cpu()))
+    flat = wide_rows(1, 64 * 8 + 1, g).cuda()[0]
+    assert same(values(ops, ops.quantize_mx4(flat[1:].view(8, 64))), plain.nearest(flat[1:].view(8, 64).cpu()))
+
+
+def test_matrices_on_top_of_one_another(ops):
+    x = wide_rows(2 * 3 * 150, 96, gen("mats")).view(2, 3, 150, 96)
+    q = ops.quantize_mx4(x.cuda())
+    assert q.codes.shape == (900, 48) and q.scales.shape == (12, 2, 512)
+    assert same(values(ops, q), plain.nearest(x))
+    y = wide_rows(900, 96, gen("mats", 2)).view(2, 3, 150, 96)
+    assert ops.quantize_mx4(y.cuda(), into=q) is q and same(values(ops, q), plain.nearest(y))
+
+
+def test_gate_and_up_lie_interleaved(ops):
+    for n in (16, 40, 129):
+        x = wide_rows(3 * 2 * n, 70, gen("pairs", n)).view(3, 2, n, 70)
+        q = ops.quantize_mx4(x.cuda(), gate_up=True)
+        full = -(-n // 16) * 32
+        assert q.codes.shape == (3 * full, 48)
+        assert same(values(ops, q), plain.nearest(x))
+        plain_q = ops.quantize_mx4(x.cuda())
+        up_5 = q.codes.view(3, full, 48)[2, 16 + 5]
+        assert torch.equal(up_5, plain_q.codes.view(3, 2, n, 48)[2, 1, 5])
+
+
+# ------------------------------------------------------------------------------------- products
+DENSE = [(1, 1, 1), (1, 128, 64), (1, 16, 32), (2, 130, 96), (16, 128, 256), (17, 200, 257), (31, 129, 1000), (32, 127, 320),
+         (33, 136, 512), (97, 40, 160), (191, 128, 64), (193, 257, 288), (385, 130, 700), (1, 300, 4096), (700, 260, 100)]
+
+
+def dense_inputs(m, n, k, mats, dtype=torch.bfloat16):
+    g = gen(m, n, k, mats)
+    a = (torch.randn(m, k, generator=g) * torch.exp(torch.randn(k, generator=g))).to(dtype)
+    w = (torch.randn(mats, n, k, generator=g) * k ** -0.5).bfloat16()
+    return a, w
+
+
+def near(got, want, off, dtype):
+    got = got.cpu().double()
+    far = (got - want).abs() - off - plain.rounding(dtype, want)
+    assert got.shape == want.shape and bool((far <= 0).all()), float(far.max())
+
+
+@pytest.mark.parametrize("m, n, k", DENSE)
+@pytest.mark.parametrize("out_dtype", [torch.bfloat16, torch.float32])
+def test_product(ops, m, n, k, out_dtype):
+    a, w = dense_inputs(m, n, k, 1)
+    out = torch.full((m, n), float("nan"), dtype=out_dtype, device="cuda")
+    ops.linear_mx4(a.cuda(), ops.prepare_weight_mx4(w[0].cuda()), out)
+    ops.check_status()
+    near(out, *plain.product(plain.nearest(a), plain.nearest(w[0])), out_dtype)
+
+
+@pytest.mark.parametrize("m, n, k", DENSE)
+@pytest.mark.parametrize("kind", ["silu", "clamped", "relu2"])
+def test_product_with_a_unit(ops, m, n, k, kind):
+    dtype = torch.float32 if (m + n + k) % 2 else torch.bfloat16
+    a, w = dense_inputs(m, n, k, 1 if kind == "relu2" else 2, dtype)
+    out = torch.full((m, n), float("nan"), dtype=dtype, device="cuda")
+    qa, qw = plain.nearest(a), plain.nearest(w)
+    if kind == "relu2":
+        ops.linear_relu_squared_mx4(a.cuda(), ops.prepare_weight_mx4(w[0].cuda()), out)
+        z, off = plain.product(qa, qw[0])
+        want, off = z.clamp(min=0) ** 2, (2 * z.clamp(min=0) + off) * off + z ** 2 * plain.STEPS
+    else:
+        alpha, limit = (1.702, 0.5) if kind == "clamped" else (1.0, 0.0)
+        ops.linear_glu_mx4(a.cuda(), ops.prepare_weight_mx4(w.cuda(), gate_up=True), out, alpha=alpha, limit=limit)
+        g, u = plain.product(qa, qw[0]), plain.product(qa, qw[1])
+        want, off = plain.unit(g[0], u[0], g[1], u[1], alpha, limit)
+    ops.check_status()
+    near(out, want, off, dtype)
+
+
+# ------------------------------------------------------------------------------------- by expert
+def routed(idx, weight, outputs):
+    """The arrays of a step in which token t takes the outputs idx[t]."""
+    flat = idx.reshape(-1)
+    order = torch.sort(flat, stable=True).indices
+    offsets = torch.searchsorted(flat[order], torch.arange(outputs + 1))
+    return {"idx": flat.int().cuda(), "order": order.int().cuda(), "offsets": offsets.int().cuda(),
+            "weight": weight.reshape(-1).cuda()}
+
+
+def choices(t, outputs, top, spread, g):
+    if spread == "one":                      # every token's first choice is the same expert
+        idx = torch.stack([torch.randperm(outputs - 1, generator=g)[:top] + 1 for _ in range(t)])
+        idx[:, 0] = 0
+        return idx
+    return torch.stack([torch.randperm(outputs, generator=g)[:top] for _ in range(t)])
+
+
+EXPERTS = [  # tokens, experts, outputs without weights, top, d, f, spread
+    (1, 3, 0, 1, 64, 16, "even"), (16, 4, 0, 1, 72, 40, "one"), (17, 4, 1, 2, 136, 128, "one"),
+    (33, 5, 0, 2, 65, 131, "one"), (65, 9, 0, 2, 257, 136, "one"), (40, 2, 0, 1, 200, 129, "even"),
+    (129, 3, 0, 2, 64, 96, "one"), (127, 2, 0, 2, 320, 264, "even"), (257, 3, 1, 2, 128, 72, "one"),
+    (600, 4, 0, 1, 64, 130, "even"), (515, 2, 0, 1, 256, 384, "one"), (70, 300, 0, 3, 64, 32, "even"),
+    (30, 1500, 3, 2, 40, 24, "even")]
+
+
+@pytest.mark.parametrize("t, experts, identity, top, d, f, spread", EXPERTS)
+@pytest.mark.parametrize("kind", ["silu", "clamped", "relu2"])
+def test_products_by_expert(ops, t, experts, identity, top, d, f, spread, kind):
+    g = gen(t, experts, kind)
+    outputs = experts + identity
+    idx = choices(t, outputs, top, spread, g)
+    weight = torch.rand(t, top, generator=g) + 0.1
+    work = routed(idx, weight, outputs)
+    dtype = torch.float32 if kind == "clamped" else torch.bfloat16
+    h = torch.randn(t, d, generator=g).to(dtype)
+    w1 = (torch.randn(experts, 1 if kind == "relu2" else 2, f, d, generator=g) * d ** -0.5).bfloat16()
+    w2 = (torch.randn(experts, d, f, generator=g) * f ** -0.5).bfloat16()
+    n = t * top
+    y = torch.full((n, f), 77.0, dtype=dtype, device="cuda")
+    out = torch.full((n, d), 77.0, device="cuda")
+    scale_in = kind == "silu"
+    if kind == "relu2":
+        ops.expert_relu_squared_mx4(h.cuda(), ops.prepare_weight_mx4(w1[:, 0].cuda()), y, work, top, scale_in)
+    else:
+        alpha, limit = (1.702, 0.5) if kind == "clamped" else (1.0, 0.0)
+        ops.expert_glu_mx4(h.cuda(), ops.prepare_weight_mx4(w1.cuda(), gate_up=True), y, work, top, scale_in, alpha=alpha,
+                           limit=limit)
+    ops.expert_down_mx4(y, ops.prepare_weight_mx4(w2.cuda()), out, work, top, not scale_in)
+    ops.check_status()
+    order, flat, share = work["order"].cpu().long(), idx.reshape(-1), weight.reshape(-1).double()
+    y, out = y.cpu(), out.cpu()
+    qh, qy = plain.nearest(h), plain.nearest(y)
+    for e in range(outputs):
+        at = (flat[order] == e).nonzero()[:, 0]
+        slot = order[at]
+        if e >= experts:
+            assert bool((y[at] == 77.0).all()) and bool((out[slot] == 77.0).all())    # nobody's: left as they were
+            continue
+        if at.numel() == 0:
+            continue
+        qw = plain.nearest(w1[e])
+        s = share[slot, None] if scale_in else torch.ones((), dtype=torch.float64)
+        sums = [plain.product(qh[slot // top], m) for m in qw]
+        sums = [(z * s, (off + z.abs() * plain.STEPS) * s) for z, off in sums]
+        if kind == "relu2":
+            z, off = sums[0]
+            want, off = z.clamp(min=0) ** 2, (2 * z.clamp(min=0) + off) * off + z ** 2 * plain.STEPS
+        else:
+            want, off = plain.unit(sums[0][0], sums[1][0], sums[0][1], sums[1][1], alpha, limit)
+        near(y[at], want, off, dtype)
+        z, off = plain.product(qy[at], plain.nearest(w2[e]))
+        s = torch.ones((), dtype=torch.float64) if scale_in else share[slot, None]
+        near(out[slot], z * s, (off + z.abs() * plain.STEPS) * s, torch.float32)
