@@ -8,6 +8,8 @@
 // product takes two at a time).
 #pragma once
 #include "common.cuh"
+#include <cuda_fp16.h>
+#include <string.h>
 
 namespace mls_mx4 {
 constexpr int BLOCK = 32;
@@ -17,7 +19,7 @@ constexpr int ATOM = 512;
 __host__ __device__ constexpr int pitch_of(int K) { return (K + BLOCK - 1) / BLOCK * (BLOCK / 2); }
 __host__ __device__ constexpr int atoms_of(int K) { return 2 * ((K + 255) / 256); }
 // Bytes from a tile's first atom to a row's four scales in its atom.
-__host__ __device__ constexpr int row_in_atom(int r) { return (r & 31) * 16 + ((r >> 5) & 3) * 4; }
+__host__ __device__ constexpr unsigned row_in_atom(unsigned r) { return (r & 31) * 16 + ((r >> 5) & 3) * 4; }
 
 // Rows of the pairs [2, N, K] of gate and up matrices lie interleaved, 16 of the gate's and 16 of up's in turn (N filled up
 // to a multiple of 16): an output's two sums are then 16 lanes of a warp apart.
@@ -26,14 +28,13 @@ __host__ __device__ constexpr int pair_row(int which, int n) { return n / 16 * 3
 
 // Where row p of matrices of N rows each lies: its row of codes, the tile of its scales and its row in that.
 struct Place {
-    long long row, tile;
-    int r;
+    unsigned row, tile, r;
 };
-__device__ __forceinline__ Place place_of(long long p, int N, bool pairs) {
-    const long long mat = p / N;
-    const int n = (int)(p - mat * N);
-    const int rows = pairs ? pair_rows(N) : N, at = pairs ? pair_row((int)(mat & 1), n) : n;
-    const long long m = pairs ? mat >> 1 : mat;
+__device__ __forceinline__ Place place_of(unsigned p, unsigned N, bool pairs) {
+    if (p < N && !pairs) return {p, p / TILE_ROWS, p % TILE_ROWS};
+    const unsigned mat = p / N, n = p - mat * N;
+    const unsigned rows = pairs ? pair_rows((int)N) : N, at = pairs ? pair_row((int)(mat & 1), (int)n) : n;
+    const unsigned m = pairs ? mat >> 1 : mat;
     return {m * rows + at, m * ((rows + TILE_ROWS - 1) / TILE_ROWS) + at / TILE_ROWS, at % TILE_ROWS};
 }
 
@@ -41,4 +42,105 @@ __device__ __forceinline__ Place place_of(long long p, int N, bool pairs) {
 // offsets[e] / 128 + e: with c rows behind offset o it takes ceil(c / 128) tiles, and (o + c) / 128 + 1 - o / 128,
 // the distance to the next expert's, is never less.
 __device__ __forceinline__ int first_tile(int offset, int e) { return offset / TILE_ROWS + e; }
+
+// Where a row that is quantised comes from and where its scales go.
+struct RowMap {
+    int rows_per_mat, pairs;                       // plain rows: matrices of so many rows, or pairs of them
+    const int *order, *idx, *offsets;              // sorted slots of a routed step (offsets == nullptr: plain rows)
+    int top, n_experts, gather;                    // gather: row p is a copy of row order[p] / top
+};
+// Rows [rows, K] of float32 or bfloat16, ld values apart, into codes and scales.
+int quantize_rows(const void* x, int dtype, long long ld, long long rows, int K, const RowMap& map, uint8_t* codes,
+                  uint8_t* scales, cudaStream_t stream);
+
+// Eight neighbouring values of a row as they lie (zeros behind the row's end); VEC: at a 16-byte place.
+template <typename T>
+struct Eight {
+    uint32_t w[2 * sizeof(T)];
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ Eight<T> load8(const T* row, int k0, int K) {
+    Eight<T> v;
+    if (VEC && k0 + 8 <= K) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            const uint4 u = reinterpret_cast<const uint4*>(row + k0)[i];
+            v.w[4 * i] = u.x, v.w[4 * i + 1] = u.y, v.w[4 * i + 2] = u.z, v.w[4 * i + 3] = u.w;
+        }
+        return v;
+    }
+    if constexpr (sizeof(T) == 2) {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            v.w[i] = (k0 + 2 * i < K ? (uint32_t)h[k0 + 2 * i] : 0u) |
+                     (k0 + 2 * i + 1 < K ? (uint32_t)h[k0 + 2 * i + 1] << 16 : 0u);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v.w[i] = k0 + i < K ? __float_as_uint(row[k0 + i]) : 0u;
+    }
+    return v;
+}
+
+// Values in [-8, 8] as codes, the first in the lowest bits.
+__device__ __forceinline__ uint32_t pack8(const float (&v)[8]) {
+    uint32_t out;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(out)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return out;
+}
+// And back: two values of a byte.
+__device__ __forceinline__ float2 unpack2(uint32_t byte) {
+    uint32_t h;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "mov.b32 {a, b, c, d}, %1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(h) : "r"(byte));
+    __half2 two;
+    memcpy(&two, &h, 4);
+    return __half22float2(two);
+}
+// The largest magnitude of three; NaN where one is none.
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
+    float m;
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(m) : "f"(a), "f"(b), "f"(c));
+    return m;
+}
+
+// A lane's eight of a warp's 256 neighbouring values as codes; four lanes share a block.  `scales` is, in lanes 0 and 16, the
+// four scales of the 128 values from that lane's on.
+//
+// A block of 32 values with the largest magnitude m has the scale 2^max(floor(log2 m) - 2, -127); a value v becomes
+// the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times the scale (a tie goes to the even code, what is larger to 6).  floor(log2 m)
+// is m's exponent field, so the scale's byte is max(field - 2, 0), and dividing by the scale is an exact product with a
+// power of two.  The bits of the largest magnitude say both the scale and, as infinities and NaN have the largest exponent
+// field, whether the block is a number at all (if not its scale is 255, whatever its codes).
+template <typename T>
+__device__ __forceinline__ uint32_t quantize8(const Eight<T>& x, int lane, uint32_t& scales) {
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        uint32_t bits;
+        if constexpr (sizeof(T) == 2) bits = j & 1 ? x.w[j / 2] & 0xffff0000u : x.w[j / 2] << 16;
+        else bits = x.w[j];
+        v[j] = __uint_as_float(bits);
+    }
+    uint32_t most = __float_as_uint(max_abs(max_abs(v[0], v[1], v[2]), max_abs(v[3], v[4], v[5]), max_abs(v[6], v[7], v[7])));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    const uint32_t field = most >> 23;
+    const uint32_t scale = field == 255 ? 255 : max(field, 2u) - 2;
+    const float inverse = __uint_as_float((254 - min(scale, 253u)) << 23);           // 2^(127 - scale)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] *= inverse;
+    scales = scale << (2 * (lane & 12));
+    scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
+    scales |= __shfl_xor_sync(0xffffffffu, scales, 8);
+    return pack8(v);
+}
 }  // namespace mls_mx4

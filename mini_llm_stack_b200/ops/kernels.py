@@ -31,6 +31,9 @@ _ERRORS = {100001: "a size this kernel does not support",
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+_MX4_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
 class KernelError(RuntimeError):
     pass
 
@@ -118,37 +121,62 @@ class Mx4:
     0.5, 1, 1.5, 2, 3, 4, 6.  ``codes``: uint8 ``[all rows, bytes]``, two codes a byte, the even place in the low bits;
     ``scales``: uint8 ``[tiles, atoms, 512]`` in the order in which they enter the tensor cores (csrc/mx4.h)."""
 
-    __slots__ = ("codes", "scales", "shape", "gate_up")
+    __slots__ = ("shape", "gate_up", "data", "lead", "n", "k", "rows", "tiles", "scales_at", "codes_at", "slice", "settled")
     TILE_ROWS = 128
 
-    def __init__(self, shape, device, gate_up: bool = False):
+    def __init__(self, shape, device, gate_up: bool = False, sm_count: int = 148):
         """Memory for matrices of this shape; ``gate_up``: pairs ``[..., 2, N, K]`` of a gate and an up matrix whose
         rows lie interleaved, 16 and 16."""
-        self.shape, self.gate_up = tuple(int(n) for n in shape), bool(gate_up)
+        self.shape, self.gate_up = tuple(shape), gate_up
         *lead, n, k = self.shape
         mats = 1
         for i in lead:
             mats *= i
+        self.lead = len(lead) - gate_up              # dimensions in front of a matrix or a pair
+        self.n, self.k = n, k
         if gate_up:
             mats, n = mats // 2, -(-n // 16) * 32
+        self.rows, self.tiles = mats * n, mats * -(-n // 128)
+        room = self.tiles * self.tile_bytes(k) + self.rows * self.pitch(k)
         # (what fills up a pair's rows is read, so it is zeroed)
-        new = torch.empty if n == self.shape[-2] or n == 2 * self.shape[-2] else torch.zeros
-        self.codes = new((mats * n, self.pitch(k)), dtype=torch.uint8, device=device)
-        self.scales = new((mats * -(-n // self.TILE_ROWS), -(-k // 256) * 2, 512), dtype=torch.uint8, device=device)
+        new = torch.zeros if gate_up and n != 2 * self.n else torch.empty
+        self.data = new(room, dtype=torch.uint8, device=device)
+        self.scales_at = self.data.data_ptr()
+        self.codes_at = self.scales_at + self.tiles * self.tile_bytes(k)
+        self.slice = self._few_rows_slice(sm_count, n, k)
+        self.settled = False          # whether the device has finished what wrote it
 
     @staticmethod
     def pitch(k: int) -> int:
         """Bytes of codes a row."""
-        return -(-k // 32) * 16
+        return (k + 31) // 32 * 16
 
     @staticmethod
     def tile_bytes(k: int) -> int:
         """Bytes of scales of 128 rows."""
-        return -(-k // 256) * 1024
+        return (k + 255) // 256 * 1024
+
+    def _few_rows_slice(self, sm_count: int, n: int, k: int) -> int:
+        """How much of K, in steps of 256, a block of the product of few rows takes: as many slices, up to eight, as leave
+        all blocks resident at once, two an SM (a block that comes in a second round costs more than its slice saves).
+        0: the tiles alone are more, the product takes the way of many rows.  (In us, this way and that one: 8 rows, 4,096
+        outputs of 14,336 in eight slices 9.3 and 20.8, 28,672 of 4,096 in one 14.4 and 17.5.  From 17 rows on one or two slices
+        do not pay: 32 rows, 28,672 of 4,096 16.9 and 16.3, 7,168 of 4,096 in four slices 8.4 and 9.3.)"""
+        steps, tiles = -(-k // 256), -(-n // 128)
+        slices = min(8, steps, 2 * sm_count * 19 // 20 // tiles)
+        return -(-steps // slices) if slices else 0
+
+    @property
+    def codes(self):
+        return self.data[self.data.numel() - self.rows * self.pitch(self.k):].view(self.rows, self.pitch(self.k))
+
+    @property
+    def scales(self):
+        return self.data[:self.tiles * self.tile_bytes(self.k)].view(self.tiles, -1, 512)
 
     @property
     def device(self):
-        return self.codes.device
+        return self.data.device
 
 
 class Ops:
@@ -188,6 +216,7 @@ class Ops:
         self._part_libs: dict = {}               # kernels of parts only some models have
         self._sample = _decl(core, "mls_sample", [_P, _P, _P, _P, _I, _I, _P, _P])
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._status_at = self.status.data_ptr()
         self._attention_libs: dict = {}
         self._attention_lib_handles: dict = {}
         self._split_ctas_per_sm: dict = {}       # head size -> CTAs of the split kernel an SM holds
@@ -958,14 +987,14 @@ class Ops:
                                     [_P, _I, _P, _I, _I, _LL, _P, _P, _I, _P, _P, _I, _P, _I, _I, _I,
                                      _P])}
         elif name == "mx4":
-            fns = {"quantize": _decl(lib, "mls_mx4_quantize",
-                                     [_P, _I, _LL, _LL, _I, _I, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P]),
+            fns = {"quantize": _decl(lib, "mls_mx4_quantize", [_P, _I, _LL, _LL, _I, _I, _I, _P, _P, _P]),
                    "values": _decl(lib, "mls_mx4_values", [_P, _P, _LL, _I, _I, _I, _P, _I, _P]),
                    "product": _decl(lib, "mls_mx4_product",
-                                    [_I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _F, _P, _P]),
+                                    [_I, _P, _I, _LL, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F,
+                                     _P, _P]),
                    "expert_product": _decl(lib, "mls_mx4_expert_product",
-                                           [_I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _I,
-                                            _F, _F, _P, _P])}
+                                           [_I, _P, _I, _LL, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I,
+                                            _P, _P, _P, _P, _I, _F, _F, _P, _P])}
         elif name == "shortconv":
             fns = {"qk": _decl(lib, "mls_qk_conv_norm_rope_store",
                                [_P, _I, _LL, _P, _P, _I, _P, _P, _I, _F, _P, _LL, _I, _P, _P, _P, _P,
@@ -1433,26 +1462,30 @@ class Ops:
             shared.release()
 
     # ------------------------------------------------- 4-bit microscaled rows and weights
-    def _mx4_source(self, x, what: str):
-        """(rows, K, row stride) of a matrix to be quantised."""
-        _need(isinstance(x, torch.Tensor) and x.dim() >= 2 and x.dtype in (torch.float32, torch.bfloat16),
-              f"{what}: rows [..., K] of float32 or bfloat16")
-        self._need_here(what, x)
-        k = x.shape[-1]
-        _need(1 <= k <= self.MX4_MOST_K, f"{what}: rows of 1 to {self.MX4_MOST_K} values, not {k}")
-        if x.dim() == 2:
-            _need(x.stride(1) == 1 or k == 1, f"{what}: a row's values must lie side by side")
-            _need(x.shape[0] <= 1 or x.stride(0) >= k, f"{what}: rows must not overlap")
-            return x.shape[0], k, max(x.stride(0), k)
-        _need(x.is_contiguous(), f"{what}: matrices must be contiguous")
-        return x.numel() // k, k, k
-
     MX4_MOST_K = 1 << 20
+    MX4_FUSED_TASKS = 64     # 256 values of a row each: with so many a block the product quantises its rows itself
 
-    def _need_here(self, what: str, *tensors) -> None:
+    def _mx4_here(self, what: str, *tensors) -> None:
         for t in tensors:
-            _need(t is None or (t.device.type == "cuda" and t.device.index == self._device_index),
-                  f"{what}: tensors must be on {self.device}")
+            if t.get_device() != self._device_index:
+                raise KernelError(f"{what}: tensors must be on {self.device}")
+        if torch.cuda.current_device() != self._device_index:
+            raise KernelError(f"{what}: {self.device} must be the current device")
+
+    @staticmethod
+    def _mx4_type(t, what: str) -> int:
+        code = _MX4_TYPES.get(t.dtype)
+        if code is None:
+            raise KernelError(f"{what}: float32 or bfloat16, not {t.dtype}")
+        return code
+
+    @staticmethod
+    def _mx4_ld(x, k: int, what: str) -> int:
+        """The distance of a matrix's rows, whose values must lie side by side."""
+        ld, step = x.stride()
+        if (step != 1 and k > 1) or (ld < k and x.shape[0] > 1):
+            raise KernelError(f"{what}: a row's values must lie side by side, rows must not overlap")
+        return ld if ld > k else k
 
     def quantize_mx4(self, x, into: Mx4 | None = None, gate_up: bool = False) -> Mx4:
         """The rows of ``x [..., rows, K]`` (float32 or bfloat16; two-dimensional ones may have a row stride) as 4-bit
@@ -1463,81 +1496,102 @@ class Ops:
         6.  A block that holds an infinity or a NaN is NaN as a whole.  The last block of a row is filled up with zeros.
         ``into``: an ``Mx4`` of the same shape to be overwritten, instead of new memory.  ``gate_up``: ``x [..., 2, N, K]``
         holds pairs of a gate and an up matrix, laid out for ``linear_glu_mx4`` and ``expert_glu_mx4``."""
-        rows, k, ld = self._mx4_source(x, "quantize_mx4")
-        _need(not gate_up or (x.dim() >= 3 and x.shape[-3] == 2), "quantize_mx4: gate_up goes with matrices [..., 2, N, K]")
+        what = "quantize_mx4"
+        shape = tuple(x.shape)
+        code = self._mx4_type(x, what)
+        if len(shape) < 2 or not 1 <= shape[-1] <= self.MX4_MOST_K:
+            raise KernelError(f"{what}: matrices [..., rows, K] with K from 1 to {self.MX4_MOST_K}, not {shape}")
+        if gate_up and (len(shape) < 3 or shape[-3] != 2):
+            raise KernelError(f"{what}: gate_up goes with matrices [..., 2, N, K], not {shape}")
+        self._mx4_here(what, x)
+        k = shape[-1]
+        if len(shape) == 2:
+            ld, rows = self._mx4_ld(x, k, what), shape[0]
+        else:
+            _need(x.is_contiguous(), "quantize_mx4: matrices must be contiguous")
+            ld, rows = k, x.numel() // k
+        gate_up = bool(gate_up)
         if into is None:
-            into = Mx4(x.shape, x.device, gate_up)
-        _need(isinstance(into, Mx4) and into.shape == tuple(x.shape) and into.gate_up == bool(gate_up),
-              "quantize_mx4: into is laid out for something else")
-        self._need_here("quantize_mx4", into.codes)
-        self._quantize_mx4(x, ld, rows, k, x.shape[-2], into.codes, into.scales, pairs=gate_up)
+            into = Mx4(shape, x.device, gate_up, self.sm_count)
+        elif into.__class__ is not Mx4 or into.shape != shape or into.gate_up != gate_up:
+            raise KernelError(f"{what}: into is laid out for something else")
+        else:
+            self._mx4_here(what, into.data)
+            into.settled = False
+        if rows:
+            self.launches += 1
+            rc = self._part_lib("mx4")["quantize"](x.data_ptr(), code, ld, rows, k, shape[-2], gate_up, into.codes_at,
+                                                   into.scales_at, self._stream())
+            if rc:
+                _check(rc, what)
         return into
-
-    def _quantize_mx4(self, x, ld, rows, k, per_mat, codes, scales, work=None, top=1, n_experts=0, gather=False,
-                      pairs=False):
-        if rows == 0:
-            return
-        self.launches += 1
-        order, idx, offsets = (work["order"], work["idx"], work["offsets"]) if work is not None else (None,) * 3
-        _check(self._part_lib("mx4")["quantize"](
-            _ptr(x), _code(x.dtype), ld, rows, k, per_mat, 1 if pairs else 0, _ptr(order), _ptr(idx), _ptr(offsets), top, n_experts,
-            1 if gather else 0, _ptr(codes), _ptr(scales), self._stream()), "quantize_mx4")
 
     def mx4_values(self, q: Mx4, out) -> None:
         """What ``q`` stands for, into ``out`` (its shape, float32 or bfloat16; both hold it exactly)."""
-        _need(isinstance(q, Mx4), "mx4_values: codes and scales of quantize_mx4")
-        _need(tuple(out.shape) == q.shape and out.is_contiguous()
-              and out.dtype in (torch.float32, torch.bfloat16), "mx4_values: bad output")
-        self._need_here("mx4_values", q.codes, out)
-        if out.numel() == 0:
-            return
-        k = q.shape[-1]
-        self.launches += 1
-        _check(self._part_lib("mx4")["values"](_ptr(q.codes), _ptr(q.scales), out.numel() // k, k, q.shape[-2],
-                                               1 if q.gate_up else 0, _ptr(out), _code(out.dtype), self._stream()),
-               "mx4_values")
+        what = "mx4_values"
+        if q.__class__ is not Mx4 or tuple(out.shape) != q.shape or not out.is_contiguous():
+            raise KernelError(f"{what}: a result of quantize_mx4 and a contiguous output of its shape")
+        code = self._mx4_type(out, what)
+        self._mx4_here(what, q.data, out)
+        rows = out.numel() // q.k
+        if rows:
+            self.launches += 1
+            rc = self._part_lib("mx4")["values"](q.codes_at, q.scales_at, rows, q.k, q.n, q.gate_up, out.data_ptr(), code,
+                                                 self._stream())
+            if rc:
+                _check(rc, what)
 
     def prepare_weight_mx4(self, w, gate_up: bool = False) -> Mx4:
         """A matrix ``[out, in]`` made ready for ``linear_mx4``, the experts' ``[E, out, in]``, or with ``gate_up`` the
         pair ``[2, out, in]`` of gate and up for ``linear_glu_mx4`` and the experts' ``[E, 2, out, in]``."""
-        return self.quantize_mx4(w.contiguous(), gate_up=gate_up)
+        held = self.quantize_mx4(w.contiguous(), gate_up=gate_up)
+        if not torch.cuda.is_current_stream_capturing():
+            # a product may ask for weights before the kernels in front of it have finished
+            torch.cuda.current_stream().synchronize()
+            held.settled = True
+        return held
 
-    def _mx4_rows(self, a, m: int, k: int, what: str):
-        """Codes and scales of a product's rows: those of an ``Mx4``, or of a tensor quantised into scratch memory."""
-        if isinstance(a, Mx4):
-            self._need_here(what, a.codes)
-            return a.codes, a.scales
-        _, _, ld = self._mx4_source(a, what)
-        pitch, tiles = Mx4.pitch(k), -(-m // Mx4.TILE_ROWS)
-        held = self.scratch("mx4_rows", (m * pitch + tiles * Mx4.tile_bytes(k)) // 4 + 4).view(torch.uint8)
-        scales = held[:tiles * Mx4.tile_bytes(k)]
-        codes = held[scales.numel():]
-        self._quantize_mx4(a, ld, m, k, m, codes, scales)
-        return codes, scales
-
-    @staticmethod
-    def _mx4_weight(w, unit: int, lead: int, what: str) -> None:
-        gated = unit == 1
-        _need(isinstance(w, Mx4) and len(w.shape) == lead + 2 + gated and w.gate_up == gated,
-              f"{what}: the weight comes from prepare_weight_mx4{' with gate_up' if gated else ''}, "
-              f"{lead + 2 + gated} dimensions")
+    def _mx4_scratch(self, m: int, k: int, tiles: int) -> tuple:
+        """Addresses of the codes and scales of a product's rows in scratch memory."""
+        scales = tiles * Mx4.tile_bytes(k)
+        held = self.scratch("mx4_rows", (m * Mx4.pitch(k) + scales) // 4)
+        at = held.data_ptr()
+        return at + scales, at
 
     def _product_mx4(self, unit: int, a, w: Mx4, out, what: str, alpha=1.0, limit=0.0) -> None:
-        self._mx4_weight(w, unit, 0, what)
-        _need(len(a.shape) == 2 and out.dim() == 2, f"{what}: shapes do not fit")
-        m, k = a.shape
-        n = w.shape[-2]
-        _need(w.shape[-1] == k and out.shape == (m, n), f"{what}: shapes do not fit")
-        _need(out.dtype in (torch.float32, torch.bfloat16) and out.is_contiguous(), f"{what}: bad output")
-        self._need_here(what, w.codes, out)
+        if w.__class__ is not Mx4 or w.lead or w.gate_up != (unit == 1):
+            raise KernelError(f"{what}: the weight comes from prepare_weight_mx4, "
+                              + ("[2, N, K] with gate_up" if unit == 1 else "[N, K]"))
+        shape, n, k = a.shape, w.n, w.k
+        m = shape[0]
+        if len(shape) != 2 or shape[1] != k or out.shape != (m, n) or not out.is_contiguous():
+            raise KernelError(f"{what}: shapes do not fit")
+        out_type = self._mx4_type(out, what)
+        ready = a.__class__ is Mx4
+        self._mx4_here(what, a.data if ready else a, w.data, out)
         if m == 0 or n == 0:
             return
-        codes, scales = self._mx4_rows(a, m, k, what)
+        rows = codes = scales = None
+        code, ld, fused = -1, 0, False
+        few = w.slice
+        if m > 16 and (m > 64 or 4 * few > -(-k // 256)):
+            few = 0
+        if ready:
+            if a.lead or a.gate_up:
+                raise KernelError(f"{what}: rows are one matrix")
+            codes, scales = a.codes_at, a.scales_at
+        else:
+            code, ld, rows = self._mx4_type(a, what), self._mx4_ld(a, k, what), a.data_ptr()
+            fused = 0 < few <= 12 and m <= 16 and m * few <= self.MX4_FUSED_TASKS
+            if not fused:
+                codes, scales = self._mx4_scratch(m, k, (m + 127) // 128)
+                self.launches += 1
         self.launches += 1
-        _check(self._part_lib("mx4")["product"](
-            unit, _ptr(codes), _ptr(scales), _ptr(w.codes), _ptr(w.scales), _ptr(out),
-            _code(out.dtype), m, n, k, float(alpha), float(limit), _ptr(self.status),
-            self._stream()), what)
+        rc = self._part_lib("mx4")["product"](unit, rows, code, ld, codes, scales, w.codes_at, w.scales_at, out.data_ptr(),
+                                              out_type, m, n, k, few, fused, w.settled, alpha, limit, self._status_at,
+                                              self._stream())
+        if rc:
+            _check(rc, what)
 
     def linear_mx4(self, a, w: Mx4, out) -> None:
         """``out[M, N] = q(a) @ w^T`` with float32 accumulation: rows and weights in 4-bit microscaled values.
@@ -1546,9 +1600,8 @@ class Ops:
         self._product_mx4(0, a, w, out, "linear_mx4")
 
     def linear_glu_mx4(self, a, w_gate_up: Mx4, out, alpha: float = 1.0, limit: float = 0.0) -> None:
-        """``out[M, N] = silu(q(a) Wg^T) * (q(a) Wu^T)`` in one kernel behind the rows' quantisation;
-        ``w_gate_up``: ``prepare_weight_mx4`` of ``[2, N, K]`` with ``gate_up``.  ``limit`` > 0: the clamped unit of
-        ``linear_clamped_glu`` instead."""
+        """``out[M, N] = silu(q(a) Wg^T) * (q(a) Wu^T)``; ``w_gate_up``: ``prepare_weight_mx4`` of ``[2, N, K]`` with
+        ``gate_up``.  ``limit`` > 0: the clamped unit of ``linear_clamped_glu`` instead."""
         self._product_mx4(1, a, w_gate_up, out, "linear_glu_mx4", alpha, limit)
 
     def linear_relu_squared_mx4(self, a, w: Mx4, out) -> None:
@@ -1557,39 +1610,40 @@ class Ops:
 
     def _expert_product_mx4(self, unit: int, rows, w: Mx4, out, work: dict, top: int, scale: bool, what: str,
                             alpha=1.0, limit=0.0) -> None:
-        self._mx4_weight(w, unit, 1, what)
-        n_experts, n, k = w.shape[0], w.shape[-2], w.shape[-1]
-        slots = out.shape[0]
-        _need(out.dim() == 2 and out.shape[1] == n and out.is_contiguous() and top >= 1 and slots % top == 0
-              and out.dtype in ((torch.float32,) if unit == 0 else (torch.float32, torch.bfloat16)),
-              f"{what}: bad output")
-        source_rows, source_k, ld = self._mx4_source(rows, what)
-        _need(rows.dim() == 2 and source_k == k and source_rows == (slots if unit == 0 else slots // top),
-              f"{what}: rows do not fit")
-        for name, dtype, least in (("order", torch.int32, slots), ("idx", torch.int32, slots),
-                                   ("offsets", torch.int32, n_experts + 1), ("weight", torch.float32, slots)):
-            held = work[name]
-            _need(held.dtype == dtype and held.is_contiguous() and held.numel() >= least, f"{what}: bad routing ({name})")
-            self._need_here(what, held)
-        self._need_here(what, w.codes, out)
+        if w.__class__ is not Mx4 or w.lead != 1 or w.gate_up != (unit == 1):
+            raise KernelError(f"{what}: the weights come from prepare_weight_mx4, "
+                              + ("[E, 2, N, K] with gate_up" if unit == 1 else "[E, N, K]"))
+        n_experts, n, k = w.shape[0], w.n, w.k
+        shape, slots = rows.shape, out.shape[0]
+        if (len(out.shape) != 2 or out.shape[1] != n or not out.is_contiguous() or len(shape) != 2 or shape[1] != k
+                or top < 1 or slots != (shape[0] if unit == 0 else shape[0] * top)):
+            raise KernelError(f"{what}: shapes do not fit")
+        code, out_type, ld = self._mx4_type(rows, what), self._mx4_type(out, what), self._mx4_ld(rows, k, what)
+        if unit == 0 and out_type:
+            raise KernelError(f"{what}: the slots' rows are float32")
+        order, idx, offsets, weight = work["order"], work["idx"], work["offsets"], work["weight"]
+        if not (order.dtype == idx.dtype == offsets.dtype == torch.int32 and weight.dtype == torch.float32
+                and order.is_contiguous() and idx.is_contiguous() and offsets.is_contiguous() and weight.is_contiguous()
+                and order.numel() >= slots and idx.numel() >= slots and weight.numel() >= slots
+                and offsets.numel() > n_experts):
+            raise KernelError(f"{what}: the routing's arrays do not fit")
+        self._mx4_here(what, rows, w.data, out, order, idx, offsets, weight)
         if slots == 0 or n_experts == 0 or n == 0:
             return
-        pitch, tiles = Mx4.pitch(k), slots // Mx4.TILE_ROWS + n_experts + 1
-        held = self.scratch("mx4_rows", (slots * pitch + tiles * Mx4.tile_bytes(k)) // 4 + 4).view(torch.uint8)
-        scales = held[:tiles * Mx4.tile_bytes(k)]
-        codes = held[scales.numel():]
-        self._quantize_mx4(rows, ld, slots, k, slots, codes, scales, work, top, n_experts, unit != 0)
-        self.launches += -(-n_experts // 1024)
-        _check(self._part_lib("mx4")["expert_product"](
-            unit, _ptr(codes), _ptr(scales), _ptr(w.codes), _ptr(w.scales), _ptr(out),
-            _code(out.dtype), slots, n_experts, n, k, _ptr(work["order"]), _ptr(work["offsets"]),
-            _ptr(work["weight"]), 1 if scale else 0, float(alpha), float(limit), _ptr(self.status), self._stream()), what)
+        codes, scales = self._mx4_scratch(slots, k, slots // 128 + n_experts + 1)
+        self.launches += 1 - (-n_experts // 1024)
+        rc = self._part_lib("mx4")["expert_product"](
+            unit, rows.data_ptr(), code, ld, top, unit != 0, codes, scales, w.codes_at, w.scales_at, out.data_ptr(), out_type,
+            slots, n_experts, n, k, order.data_ptr(), idx.data_ptr(), offsets.data_ptr(), weight.data_ptr(), scale, alpha,
+            limit, self._status_at, self._stream())
+        if rc:
+            _check(rc, what)
 
     def expert_glu_mx4(self, h, w_gate_up: Mx4, y, work: dict, top: int, scale_in: bool,
                        alpha: float = 1.0, limit: float = 0.0) -> None:
         """``expert_glu`` with 4-bit microscaled rows and weights; ``w_gate_up``: ``prepare_weight_mx4`` of
-        ``[E, 2, F, K]`` with ``gate_up``.  With ``scale_in`` a slot's weight multiplies the two float32 sums (the rows are quantised
-        without it).  Rows of ``y`` behind the last expert's are left as they are."""
+        ``[E, 2, F, K]`` with ``gate_up``.  With ``scale_in`` a slot's weight multiplies the two float32 sums (the rows
+        are quantised without it).  Rows of ``y`` behind the last expert's are left as they are."""
         self._expert_product_mx4(1, h, w_gate_up, y, work, top, scale_in, "expert_glu_mx4", alpha, limit)
 
     def expert_relu_squared_mx4(self, h, w_up: Mx4, y, work: dict, top: int, scale_in: bool) -> None:
