@@ -65,6 +65,29 @@ mx4_quantize_kernel(const T* __restrict__ x, long long ld, const Tasks tasks, in
     }
 }
 
+// The sorted slot p of a routed step gets the codes and scales of its token: a warp a slot, 16 bytes of codes and four of scales a
+// lane at a time.
+__global__ void __launch_bounds__(256)
+mx4_spread_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int slots, int K, const RowMap map,
+                  uint8_t* __restrict__ to_codes, uint8_t* __restrict__ to_scales) {
+    chain_release();
+    chain_wait();
+    const int p = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (p >= slots) return;
+    const int slot = map.order[p], e = map.idx[slot];
+    if (e >= map.n_experts) return;                  // a slot of an output without weights: nobody reads it
+    const int token = slot / map.top, o = map.offsets[e], pieces = pitch_of(K) / 16, atoms = atoms_of(K);
+    const uint4* from = reinterpret_cast<const uint4*>(codes) + (size_t)token * pieces;
+    uint4* to = reinterpret_cast<uint4*>(to_codes) + (size_t)p * pieces;
+#pragma unroll 4
+    for (int i = lane; i < pieces; i += 32) to[i] = from[i];
+    const uint8_t* sf = scales + (size_t)(token / TILE_ROWS) * atoms * ATOM + row_in_atom(token % TILE_ROWS);
+    uint8_t* to_sf = to_scales + (size_t)(first_tile(o, e) + (p - o) / TILE_ROWS) * atoms * ATOM +
+                     row_in_atom((p - o) % TILE_ROWS);
+    for (int i = lane; i < atoms; i += 32)
+        *reinterpret_cast<uint32_t*>(to_sf + (size_t)i * ATOM) = *reinterpret_cast<const uint32_t*>(sf + (size_t)i * ATOM);
+}
+
 // What codes and scales stand for, in the same tasks.  A lane takes PER neighbouring values, 16 bytes of output, once in 256
 // bfloat16 values and twice in 256 of float32 (two stores of 16 bytes a lane, 32 apart from the next lane's: 62 us for
 // 14,336 x 4,096 instead of 43).
@@ -149,25 +172,28 @@ bool tasks_of(long long rows, int K, Tasks& tasks, unsigned& blocks) {
 
 template <typename T>
 int quantize(const void* x, long long ld, long long rows, int K, const RowMap& map, uint8_t* codes, uint8_t* scales,
-             cudaStream_t stream) {
+             bool chained, cudaStream_t stream) {
     Tasks tasks;
     unsigned blocks;
     if (!tasks_of(rows, K, tasks, blocks)) return MLS_ERR_UNSUPPORTED;
-    if (aligned16(x) && ld % (16 / (int)sizeof(T)) == 0)
-        MLS_LAUNCH((mx4_quantize_kernel<T, true>), dim3(blocks), dim3(256), 0, stream, (const T*)x, ld, tasks, K,
-                   map, codes, scales);
-    else
-        MLS_LAUNCH((mx4_quantize_kernel<T, false>), dim3(blocks), dim3(256), 0, stream, (const T*)x, ld, tasks, K,
-                   map, codes, scales);
-    return launch_status();
+    auto* kernel = aligned16(x) && ld % (16 / (int)sizeof(T)) == 0 ? mx4_quantize_kernel<T, true> : mx4_quantize_kernel<T, false>;
+    const int rc = chained ? launch_chained(kernel, dim3(blocks), dim3(256), 0, stream, (const T*)x, ld, tasks, K, map, codes, scales)
+                           : launch_plain(kernel, dim3(blocks), dim3(256), 0, stream, (const T*)x, ld, tasks, K, map, codes, scales);
+    return rc ? rc : launch_status();
 }
 }  // namespace
 
 namespace mls_mx4 {
 int quantize_rows(const void* x, int dtype, long long ld, long long rows, int K, const RowMap& map, uint8_t* codes,
-                  uint8_t* scales, cudaStream_t stream) {
-    return dtype == MLS_BF16 ? quantize<__nv_bfloat16>(x, ld, rows, K, map, codes, scales, stream)
-                             : quantize<float>(x, ld, rows, K, map, codes, scales, stream);
+                  uint8_t* scales, bool chained, cudaStream_t stream) {
+    return dtype == MLS_BF16 ? quantize<__nv_bfloat16>(x, ld, rows, K, map, codes, scales, chained, stream)
+                             : quantize<float>(x, ld, rows, K, map, codes, scales, chained, stream);
+}
+int spread_rows(const uint8_t* codes, const uint8_t* scales, long long slots, int K, const RowMap& map, uint8_t* to_codes,
+                uint8_t* to_scales, cudaStream_t stream) {
+    const int rc = launch_plain(mx4_spread_kernel, dim3((unsigned)((slots + 7) / 8)), dim3(256), 0, stream, codes, scales,
+                                (int)slots, K, map, to_codes, to_scales);
+    return rc ? rc : launch_status();
 }
 }  // namespace mls_mx4
 
@@ -177,7 +203,7 @@ MLS_API int mls_mx4_quantize(const void* x, int dtype, long long ld, long long r
     if (rows <= 0) return 0;
     if (K <= 0 || rows_per_mat <= 0) return MLS_ERR_UNSUPPORTED;
     const RowMap map{rows_per_mat, pairs, nullptr, nullptr, nullptr, 1, 0, 0};
-    return quantize_rows(x, dtype, ld, rows, K, map, (uint8_t*)codes, (uint8_t*)scales, (cudaStream_t)stream);
+    return quantize_rows(x, dtype, ld, rows, K, map, (uint8_t*)codes, (uint8_t*)scales, true, (cudaStream_t)stream);
 }
 
 MLS_API int mls_mx4_values(const void* codes, const void* scales, long long rows, int K, int rows_per_mat, int pairs,

@@ -49,9 +49,24 @@ struct RowMap {
     const int *order, *idx, *offsets;              // sorted slots of a routed step (offsets == nullptr: plain rows)
     int top, n_experts, gather;                    // gather: row p is a copy of row order[p] / top
 };
+// A launch that starts when the kernels before it have finished.
+template <typename... Params, typename... Args>
+static inline int launch_plain(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                               Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 // Rows [rows, K] of float32 or bfloat16, ld values apart, into codes and scales.
 int quantize_rows(const void* x, int dtype, long long ld, long long rows, int K, const RowMap& map, uint8_t* codes,
-                  uint8_t* scales, cudaStream_t stream);
+                  uint8_t* scales, bool chained, cudaStream_t stream);
+// Rows that are codes and scales already, gathered into the sorted slots of a routed step (map.gather).
+int spread_rows(const uint8_t* codes, const uint8_t* scales, long long slots, int K, const RowMap& map, uint8_t* to_codes,
+                uint8_t* to_scales, cudaStream_t stream);
 
 // Eight neighbouring values of a row as they lie (zeros behind the row's end); VEC: at a 16-byte place.
 template <typename T>

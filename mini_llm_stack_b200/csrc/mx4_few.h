@@ -178,16 +178,8 @@ __device__ __forceinline__ void few_block(const FewProduct& p, const CUtensorMap
             const uint32_t sf_a = tmem_base + L::SF_AT + slot * L::SF_COLS_STAGE, sf_b = sf_a + SF_COLS;
             const int steps = min(4, (p.K - (kb0 + g) * BK + 63) / 64);
             if (elect_one()) {
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    copy_atom(sf_a + x * 4, atom_desc(a + UMMA_M * CODE_ROW + x * ATOM));
-                    copy_atom(sf_b + x * 4, atom_desc(b + NR * CODE_ROW + x * ATOM));
-                }
-#pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                    if (kk < steps)
-                        umma_mx4(tmem_base, umma_desc(a + kk * 32), umma_desc(b + kk * 32), kk & 1 ? idesc1 : idesc0,
-                                 sf_a + (kk >> 1) * 4, sf_b + (kk >> 1) * 4, (g | kk) ? 1u : 0u);
+                copy_scales<false, 1>(sf_a, sf_b, atom_desc(a + UMMA_M * CODE_ROW), atom_desc(b + NR * CODE_ROW));
+                multiply_stage<false, 1>(tmem_base, umma_desc(a), umma_desc(b), idesc0, idesc1, sf_a, sf_b, g > 0, steps);
                 umma_commit(empty(slot));
             }
             __syncwarp();
@@ -244,7 +236,8 @@ __device__ __forceinline__ void few_block(const FewProduct& p, const CUtensorMap
                 v += load_cluster_f32(at, s);
                 if (pairs) u += load_cluster_f32(at + 64, s);
             }
-            if (pairs) v = mls_experts::gated_unit(v, u, p.alpha, p.limit);
+            if (pairs) v = p.out_type == MLS_BF16 ? unit_of_sums<__nv_bfloat16>(v, u, p.alpha, p.limit)
+                                                  : unit_of_sums<float>(v, u, p.alpha, p.limit);
             else if (p.unit == RELU2) v = fmaxf(v, 0.f) * fmaxf(v, 0.f);
             store_from_float(p.out, (size_t)r * p.width + n, p.out_type, v);
         }

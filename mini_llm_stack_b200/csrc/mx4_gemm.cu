@@ -17,6 +17,7 @@
 // tensor memory and returns.
 #include "mx4_few.h"
 #include "mx4_gemm.h"
+#include "mx4_pair.h"
 #include <map>
 #include <mutex>
 #include <tuple>
@@ -31,6 +32,13 @@ mx4_product_kernel(const Product p, const __grid_constant__ CUtensorMap rows_map
     product_block<NT, GROUPED>(p, &rows_map, &w_map);
 }
 
+template <int NT, bool GROUPED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairPlan<NT, GROUPED>::THREADS), 1)
+mx4_pair_kernel(const Product p, const __grid_constant__ CUtensorMap m_map, const __grid_constant__ CUtensorMap n_map,
+                const __grid_constant__ CUtensorMap sf_m_map, const __grid_constant__ CUtensorMap sf_n_map) {
+    pair_block<NT, GROUPED>(p, &m_map, &n_map, &sf_m_map, &sf_n_map);
+}
+
 template <int NR, bool FUSED>
 __global__ void __launch_bounds__(FEW_THREADS)
 mx4_few_kernel(const FewProduct p, const __grid_constant__ CUtensorMap rows_map, const __grid_constant__ CUtensorMap w_map) {
@@ -41,33 +49,52 @@ mx4_few_kernel(const FewProduct p, const __grid_constant__ CUtensorMap rows_map,
 struct MapKey {
     const void* ptr;
     long long rows;
-    int k, box_rows;
+    int k, box, kind;
     bool operator<(const MapKey& o) const {
-        return std::tie(ptr, rows, k, box_rows) < std::tie(o.ptr, o.rows, o.k, o.box_rows);
+        return std::tie(ptr, rows, k, box, kind) < std::tie(o.ptr, o.rows, o.k, o.box, o.kind);
     }
 };
-bool codes_map(const void* ptr, long long rows, int K, int box_rows, CUtensorMap* out) {
+template <typename Encode>
+bool kept_map(const MapKey& key, CUtensorMap* out, Encode encode) {
     static std::map<MapKey, CUtensorMap> maps;
     static std::mutex lock;
     std::lock_guard<std::mutex> guard(lock);
-    const MapKey key{ptr, rows, K, box_rows};
     auto it = maps.find(key);
     if (it == maps.end()) {
         if (maps.size() > 4096) maps.clear();
         EncodeTiledFn fn = encode_fn();
-        if (!fn) return false;
         CUtensorMap m;
-        const cuuint64_t size[2] = {(cuuint64_t)pitch_of(K), (cuuint64_t)rows}, stride[1] = {(cuuint64_t)pitch_of(K)};
-        const cuuint32_t box[2] = {CODE_ROW, (cuuint32_t)box_rows}, step[2] = {1, 1};
-        if (fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), size, stride, box, step,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-            return false;
+        if (!fn || encode(fn, &m) != CUDA_SUCCESS) return false;
         it = maps.emplace(key, m).first;
     }
     *out = it->second;
     return true;
 }
+// Codes [rows, pitch] in boxes of box_rows x 128 bytes.
+bool codes_map(const void* ptr, long long rows, int K, int box_rows, CUtensorMap* out) {
+    return kept_map({ptr, rows, K, box_rows, 0}, out, [&](EncodeTiledFn fn, CUtensorMap* m) {
+        const cuuint64_t size[2] = {(cuuint64_t)pitch_of(K), (cuuint64_t)rows}, stride[1] = {(cuuint64_t)pitch_of(K)};
+        const cuuint32_t box[2] = {(cuuint32_t)CODE_ROW, (cuuint32_t)box_rows}, step[2] = {1, 1};
+        return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(ptr), size, stride, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
+}
+// Scales [tiles, stages of K, 1,024 bytes] in boxes of the same stage of box_tiles tiles.
+bool scales_map(const void* ptr, long long tiles, int K, int box_tiles, CUtensorMap* out) {
+    return kept_map({ptr, tiles, K, box_tiles, 1}, out, [&](EncodeTiledFn fn, CUtensorMap* m) {
+        const cuuint64_t stages = (K + BK - 1) / BK;
+        const cuuint64_t size[3] = {SF_STAGE / 4, stages, (cuuint64_t)tiles}, stride[2] = {SF_STAGE, stages * SF_STAGE};
+        const cuuint32_t box[3] = {SF_STAGE / 4, 1, (cuuint32_t)box_tiles}, step[3] = {1, 1, 1};
+        return fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<void*>(ptr), size, stride, box, step,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
+}
+
+// Products of many rows are long: their kernels start when the ones before have finished, as those of a step of many tokens
+// do (common.cuh).  Those of fewer rows are chained if all blocks that quantise them are resident at once.
+bool chained(long long rows, int K) { return rows <= 256 && rows * ((K + 255) / 256) <= 32LL * sm_count(); }
 
 template <int NT, bool GROUPED>
 int launch_nt(const Product& p, const void* rows, const void* W, cudaStream_t stream) {
@@ -90,14 +117,75 @@ int launch_nt(const Product& p, const void* rows, const void* W, cudaStream_t st
     const long long units = tiles * ((p.N + UMMA_M - 1) / UMMA_M);
     if (units > 0x7fffffffLL) return MLS_ERR_UNSUPPORTED;
     const int grid = (int)(units < sm_count() ? units : sm_count());
-    MLS_LAUNCH((mx4_product_kernel<NT, GROUPED>), dim3(grid), dim3(THREADS),
-               L::FIXED + (GROUPED ? 4 * (p.n_experts + 1) : 0), stream, p, rows_map, w_map);
-    return launch_status();
+    const size_t smem = L::FIXED + (GROUPED ? 4 * (p.n_experts + 1) : 0);
+    const int rc = chained(p.M, p.K)
+                       ? launch_chained(mx4_product_kernel<NT, GROUPED>, dim3(grid), dim3(THREADS), smem, stream, p, rows_map, w_map)
+                       : launch_plain(mx4_product_kernel<NT, GROUPED>, dim3(grid), dim3(THREADS), smem, stream, p, rows_map, w_map);
+    return rc ? rc : launch_status();
 }
 
+template <int NT, bool GROUPED>
+int launch_pair(const Product& p, const void* rows, const void* W, cudaStream_t stream) {
+    using L = PairPlan<NT, GROUPED>;
+    static bool configured = false;
+    if (!configured) {
+        const cudaError_t e = cudaFuncSetAttribute(mx4_pair_kernel<NT, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   L::FIXED + 4 * (TABLE_EXPERTS + 1));
+        if (e != cudaSuccess) return (int)e;
+        configured = true;
+    }
+    const long long row_tiles = GROUPED ? p.M / TILE_ROWS + p.all_experts + 1 : (p.M + TILE_ROWS - 1) / TILE_ROWS;
+    const long long w_tiles = (long long)p.n_experts * ((p.N + TILE_ROWS - 1) / TILE_ROWS);
+    CUtensorMap rows_map, w_map, sf_rows_map, sf_w_map;
+    if (!codes_map(rows, p.M, p.K, GROUPED ? L::BOX : UMMA_M, &rows_map) ||
+        !codes_map(W, (long long)p.n_experts * p.N, p.K, GROUPED ? UMMA_M : L::BOX, &w_map) ||
+        !scales_map(p.sf_a, row_tiles, p.K, GROUPED ? 2 : 1, &sf_rows_map) ||
+        !scales_map(p.sf_w, w_tiles, p.K, GROUPED ? 1 : 2, &sf_w_map))
+        return MLS_ERR_TENSOR_MAP;
+    constexpr int ROW_TILE = GROUPED ? NT : L::MT, W_TILE = GROUPED ? L::MT : NT;
+    const long long tiles = GROUPED ? (long long)(p.M / ROW_TILE) + (p.M < p.n_experts ? p.M : p.n_experts)
+                                    : (long long)(p.M + ROW_TILE - 1) / ROW_TILE;
+    const long long units = tiles * ((p.N + W_TILE - 1) / W_TILE);
+    if (units > 0x3fffffffLL) return MLS_ERR_UNSUPPORTED;
+    const int most = sm_count() / 2, pairs = (int)(units < most ? units : most);
+    const size_t smem = L::FIXED + (GROUPED ? 4 * (p.n_experts + 1) : 0);
+    const int rc = GROUPED ? launch_plain(mx4_pair_kernel<NT, GROUPED>, dim3(2 * pairs), dim3(L::THREADS), smem, stream, p, w_map,
+                                          rows_map, sf_w_map, sf_rows_map)
+                           : launch_plain(mx4_pair_kernel<NT, GROUPED>, dim3(2 * pairs), dim3(L::THREADS), smem, stream, p,
+                                          rows_map, w_map, sf_rows_map, sf_w_map);
+    return rc ? rc : launch_status();
+}
+
+// The ways of many rows, by the tile of a unit of work: 128 weights x 64 or 192 rows on one block, 256 rows x 192 or 256 weights on
+// a pair.  Units are dealt out in rounds of one a block or pair; a round takes so long for every 256 of K, and so long for what
+// its epilogue leaves visible.  The cheapest way is taken.  Measured, us, in the order 64 / 192 / 192 on pairs / 256 on pairs:
+//   256 rows x 14,336, 4,096 outputs       21.4 / 29.1 / 23.5 / 22.7     2,048 rows          125 / 81 / 62 / 45
+//   192 x 4,096, 28,672 gated              29 / 19.5 / 22 / 18.7         384 rows            55 / 34.5 / 34.0 / 36.0
+//   707 x 2,048, 16,384 gated              35 / 22.1 / 19.4 / 20.5       2,048 rows          84 / 48 / 40 / 44
+//   256 x 2,048, 2,048                     5.9 / 9.1 / 8.4 / 9.1         2,048 rows          15.7 / 14.1 / 12.9 / 9.9
 template <bool GROUPED>
-int launch(const Product& p, const void* rows, const void* W, int average, cudaStream_t stream) {
-    return average > 32 ? launch_nt<192, GROUPED>(p, rows, W, stream) : launch_nt<64, GROUPED>(p, rows, W, stream);
+int launch(const Product& p, const void* rows, const void* W, cudaStream_t stream) {
+    const double k = (p.K + BK - 1) / BK, gated = p.unit == GATED ? 1 : 0;
+    // (routed: experts of somewhat more than the average number of rows)
+    const long long experts = p.M < p.n_experts ? p.M : p.n_experts;
+    const long long each = GROUPED ? (p.M / experts * 11 + 9) / 10 + 1 : p.M;
+    const long long sets = GROUPED ? experts : 1;
+    auto cost = [&](long long row_tile, long long w_tile, int places, double per_k, double rest) {
+        const long long units = sets * ((each + row_tile - 1) / row_tile) * ((p.N + w_tile - 1) / w_tile);
+        return (double)((units + places - 1) / places) * (k * per_k + rest);
+    };
+    const int blocks = sm_count(), pairs = blocks / 2;
+    const double t[4] = {cost(64, 128, blocks, 0.335, 0.45),
+                         cost(192, 128, blocks, 0.30 + 0.00094 * (double)(each < 192 ? each : 192), 0.8),
+                         GROUPED ? 1e30 : cost(256, 192, pairs, 0.40, 0.3),
+                         cost(256, 256, pairs, 0.375, 1.3 + 1.2 * gated)};
+    int best = 0;
+    for (int way = 1; way < 4; ++way)
+        if (t[way] < t[best]) best = way;
+    return best == 0   ? launch_nt<64, GROUPED>(p, rows, W, stream)
+           : best == 1 ? launch_nt<192, GROUPED>(p, rows, W, stream)
+           : best == 2 ? launch_pair<(GROUPED ? 256 : 192), GROUPED>(p, rows, W, stream)
+                       : launch_pair<256, GROUPED>(p, rows, W, stream);
 }
 
 template <int NR, bool FUSED>
@@ -134,7 +222,7 @@ MLS_API int mls_mx4_product(int unit, const void* rows, int rows_type, long long
     if (rows_type < 0 || slice <= 0) fused = 0;
     if (rows_type >= 0 && !fused) {
         const int rc = quantize_rows(rows, rows_type, ld, M, K, RowMap{M, 0, nullptr, nullptr, nullptr, 1, 0, 0}, (uint8_t*)a,
-                                     (uint8_t*)sf_a, stream);
+                                     (uint8_t*)sf_a, chained(M, K), stream);
         if (rc) return rc;
     }
     if (slice > 0) {
@@ -151,20 +239,30 @@ MLS_API int mls_mx4_product(int unit, const void* rows, int rows_type, long long
                          : launch_few<64, false>(p, a, w, stream);
     }
     const Product p{out, (const uint8_t*)sf_w, (const uint8_t*)sf_a, nullptr, nullptr, nullptr, unit, 0, out_type,
-                    1, 0, M, w_rows, K, N, alpha, limit, status};
-    return launch<false>(p, a, w, M > 64 ? M : 0, stream);
+                    1, 0, 1, M, w_rows, K, N, alpha, limit, status};
+    return launch<false>(p, a, w, stream);
 }
 
 // Expert by expert: the slots of a routed step and w [E, 1 or 2, N, K].  The rows (sorted, or gathered from the tokens')
-// are quantised into a and sf_a first.
-MLS_API int mls_mx4_expert_product(int unit, const void* rows, int rows_type, long long ld, int top, int gather, void* a,
-                                   void* sf_a, const void* w, const void* sf_w, void* out, int out_type, int n_slots,
-                                   int n_experts, int N, int K, const int* order, const int* idx, const int* offsets,
-                                   const float* weight, int scale, float alpha, float limit, int* status, void* stream) {
+// are quantised into a and sf_a first: `tokens` rows once each into t and sf_t and from there into their slots, or (tokens == 0)
+// every slot's by itself.
+MLS_API int mls_mx4_expert_product(int unit, const void* rows, int rows_type, long long ld, int top, int gather, int tokens,
+                                   void* t, void* sf_t, void* a, void* sf_a, const void* w, const void* sf_w, void* out,
+                                   int out_type, int n_slots, int n_experts, int N, int K, const int* order, const int* idx,
+                                   const int* offsets, const float* weight, int scale, float alpha, float limit, int* status,
+                                   void* stream_) {
     if (n_slots <= 0 || N <= 0 || n_experts <= 0) return 0;
     if (K <= 0 || top <= 0) return MLS_ERR_UNSUPPORTED;
-    const int rc = quantize_rows(rows, rows_type, ld, n_slots, K, RowMap{n_slots, 0, order, idx, offsets, top, n_experts, gather},
-                                 (uint8_t*)a, (uint8_t*)sf_a, (cudaStream_t)stream);
+    const cudaStream_t stream = (cudaStream_t)stream_;
+    const RowMap map{n_slots, 0, order, idx, offsets, top, n_experts, gather};
+    int rc;
+    if (tokens > 0) {
+        rc = quantize_rows(rows, rows_type, ld, tokens, K, RowMap{tokens, 0, nullptr, nullptr, nullptr, 1, 0, 0}, (uint8_t*)t,
+                           (uint8_t*)sf_t, false, stream);
+        if (!rc) rc = spread_rows((const uint8_t*)t, (const uint8_t*)sf_t, n_slots, K, map, (uint8_t*)a, (uint8_t*)sf_a, stream);
+    } else {
+        rc = quantize_rows(rows, rows_type, ld, n_slots, K, map, (uint8_t*)a, (uint8_t*)sf_a, chained(n_slots, K), stream);
+    }
     if (rc) return rc;
     const int w_rows = unit == GATED ? pair_rows(N) : N;         // of an expert's weights
     // as many experts a launch as their table has room beside the stages
@@ -172,9 +270,8 @@ MLS_API int mls_mx4_expert_product(int unit, const void* rows, int rows_type, lo
         const int n = n_experts - e0 < TABLE_EXPERTS ? n_experts - e0 : TABLE_EXPERTS;
         const size_t tiles = (size_t)e0 * ((w_rows + TILE_ROWS - 1) / TILE_ROWS);
         const Product p{out, (const uint8_t*)sf_w + tiles * atoms_of(K) * ATOM, (const uint8_t*)sf_a, order, offsets + e0,
-                        weight, unit, scale, out_type, n, e0, n_slots, w_rows, K, N, alpha, limit, status};
-        const int rc = launch<true>(p, a, (const uint8_t*)w + (size_t)e0 * w_rows * pitch_of(K), n_slots / n_experts,
-                                    (cudaStream_t)stream);
+                        weight, unit, scale, out_type, n, e0, n_experts, n_slots, w_rows, K, N, alpha, limit, status};
+        rc = launch<true>(p, a, (const uint8_t*)w + (size_t)e0 * w_rows * pitch_of(K), stream);
         if (rc) return rc;
     }
     return 0;

@@ -49,6 +49,55 @@ __device__ __forceinline__ void umma_mx4(uint32_t tmem_d, uint64_t adesc, uint64
         ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sf_a), "r"(sf_b), "r"(accumulate) : "memory");
 }
 
+// For a pair of blocks (cta_group::2): both blocks' copies from their own shared memory, one instruction for both.
+__device__ __forceinline__ void copy_atom_pair(uint32_t tmem, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void umma_mx4_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                              uint32_t sf_a, uint32_t sf_b, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sf_a), "r"(sf_b), "r"(accumulate) : "memory");
+}
+
+// The scales of a stage into tensor memory: A's tile of 128 rows to sf_a, B's TILES to sf_b, sub-columns of 128 of K side by side for
+// B.  `scales`: descriptor of A's first atom; B's follow A's.
+template <bool PAIR, int TILES>
+__device__ __forceinline__ void copy_scales(uint32_t sf_a, uint32_t sf_b, uint64_t scales_a, uint64_t scales_b) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        if (PAIR) copy_atom_pair(sf_a + x * 4, scales_a + x * (ATOM >> 4));
+        else copy_atom(sf_a + x * 4, scales_a + x * (ATOM >> 4));
+#pragma unroll
+        for (int j = 0; j < TILES; ++j) {
+            const uint64_t from = scales_b + (j * SF_STAGE + x * ATOM >> 4);
+            if (PAIR) copy_atom_pair(sf_b + (x * TILES + j) * 4, from);
+            else copy_atom(sf_b + (x * TILES + j) * 4, from);
+        }
+    }
+}
+// The instructions of a stage: 64 of K each, `steps` of them (fewer than four only at the end of K), onto d or, at the start, in its
+// place.  a, b: descriptors of the operands' first 64 of K.
+template <bool PAIR, int TILES>
+__device__ __forceinline__ void multiply_stage(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc0, uint32_t idesc1,
+                                               uint32_t sf_a, uint32_t sf_b, bool onto, int steps) {
+    auto one = [&](int kk) {
+        const uint32_t idesc = kk & 1 ? idesc1 : idesc0, sa = sf_a + (kk >> 1) * 4, sb = sf_b + (kk >> 1) * (TILES * 4);
+        if (PAIR) umma_mx4_pair(d, a + kk * 2, b + kk * 2, idesc, sa, sb, (onto || kk) ? 1u : 0u);
+        else umma_mx4(d, a + kk * 2, b + kk * 2, idesc, sa, sb, (onto || kk) ? 1u : 0u);
+    };
+    if (steps == 4) {
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) one(kk);
+    } else {
+#pragma unroll
+        for (int kk = 0; kk < 3; ++kk)
+            if (kk < steps) one(kk);
+    }
+}
+
 constexpr int pow2_at_least(int n) { return n <= 32 ? 32 : n <= 64 ? 64 : n <= 128 ? 128 : n <= 256 ? 256 : 512; }
 
 constexpr int TABLE_EXPERTS = 1024;                  // experts of a launch: their table lies beside the stages
@@ -90,7 +139,8 @@ struct Product {
     const int *order, *offsets;                      // a routed step's (nullptr: one matrix)
     const float* weight;
     int unit, scale, out_type;                       // unit: DOWN, GATED, RELU2
-    int n_experts, first_expert, M, N, K;            // N: rows of a weight matrix, a pair's 32 for 16 outputs
+    int n_experts, first_expert, all_experts;        // of this launch, of the step
+    int M, N, K;                                     // N: rows of a weight matrix, a pair's 32 for 16 outputs
     int width;                                       // outputs of a row
     float alpha, limit;
     int* status;
@@ -101,11 +151,12 @@ struct Product {
 struct Unit {
     int e, n0, row0, rows, sf_tile, sf_row;
 };
-template <int NT, bool GROUPED>
+// ROWS: rows of weights of a unit, of which there are m_tiles times as many.
+template <int NT, bool GROUPED, int ROWS = UMMA_M>
 __device__ __forceinline__ Unit unit_of(const Product& p, int i, int m_tiles, const int* start) {
     if (!GROUPED) {
         const int tiles = (p.M + NT - 1) / NT, m = i / tiles, at = (i - m * tiles) * NT;
-        return {0, m * UMMA_M, at, min(NT, p.M - at), at / TILE_ROWS, at % TILE_ROWS};
+        return {0, m * ROWS, at, min(NT, p.M - at), at / TILE_ROWS, at % TILE_ROWS};
     }
     const int q = i / m_tiles;
     int lo = 0, hi = p.n_experts;                    // start[lo] <= q < start[hi]
@@ -117,8 +168,142 @@ __device__ __forceinline__ Unit unit_of(const Product& p, int i, int m_tiles, co
     const int tiles = start[lo + 1] - start[lo], j = i - start[lo] * m_tiles;
     const int m = j / tiles, at = (j - m * tiles) * NT;
     const int p0 = p.offsets[lo], count = p.offsets[lo + 1] - p0;
-    return {lo, m * UMMA_M, p0 + at, min(NT, count - at), first_tile(p0, p.first_expert + lo) + at / TILE_ROWS,
+    return {lo, m * ROWS, p0 + at, min(NT, count - at), first_tile(p0, p.first_expert + lo) + at / TILE_ROWS,
             at % TILE_ROWS};
+}
+
+// start[e]: row tiles of the experts before e.  A lane takes neighbouring experts, whose loads are under way together.
+template <int NT>
+__device__ __forceinline__ void row_tiles(const Product& p, int lane, int* start) {
+    const int per = (p.n_experts + 31) / 32, e0 = min(lane * per, p.n_experts), e1 = min(e0 + per, p.n_experts);
+    int sum = 0, at = e0 < e1 ? p.offsets[e0] : 0;
+#pragma unroll 8
+    for (int e = e0; e < e1; ++e) {
+        const int next = p.offsets[e + 1];
+        sum += (next - at + NT - 1) / NT;
+        at = next;
+    }
+    int before = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
+    }
+    if (lane == 31) start[p.n_experts] = before;
+    before -= sum;
+    at = e0 < e1 ? p.offsets[e0] : 0;
+#pragma unroll 8
+    for (int e = e0; e < e1; ++e) {
+        const int next = p.offsets[e + 1];
+        start[e] = before;
+        before += (next - at + NT - 1) / NT;
+        at = next;
+    }
+}
+
+// The gated unit on two sums on its way to 16 bits: exponential and reciprocal by the approximations of the special function
+// unit, whose 2^-21 or so vanish in the rounding to 2^-8 (the unit of 2,048 x 14,336 outputs in float32's precision kept the
+// product of K = 2,048 waiting: 55 us instead of XXX).  Outputs of 32 bits take the precise one.
+template <typename OUT>
+__device__ __forceinline__ float unit_of_sums(float g, float u, float alpha, float limit) {
+    if (sizeof(OUT) == 4) return mls_experts::gated_unit(g, u, alpha, limit);
+    float z = g;
+    if (limit > 0.f) {
+        g = fminf(g, limit);
+        u = fminf(fmaxf(u, -limit), limit) + 1.0f;
+        z = alpha * g;
+    }
+    float e, r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(z * -1.4426950408889634f));
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return g * r * u;
+}
+
+// Where the rows of a warp's runs of 16 go (lane x of the first 16 holds row x), and the weights of their slots: read while the
+// instructions still run.
+template <int RUNS>
+struct Rows {
+    int to[RUNS];
+    float share[RUNS];
+};
+template <bool GROUPED, int RUNS>
+__device__ __forceinline__ Rows<RUNS> rows_of(const Product& p, const Unit& u, int set, int sets, int lane) {
+    Rows<RUNS> r;
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+        const int x = (i * sets + set) * 16 + lane;
+        r.to[i] = u.row0 + x;
+        r.share[i] = 1.f;
+        if (GROUPED && (p.unit == DOWN || p.scale) && lane < 16 && x < u.rows) {
+            const int s = p.order[r.to[i]];
+            if (p.scale) r.share[i] = p.weight[s];
+            if (p.unit == DOWN) r.to[i] = s;
+        }
+    }
+    return r;
+}
+// A unit's sums on their way out: a warp takes the quarter q of the lanes (32 of the 128 rows of weights) and its set's runs of 16
+// of the batch's rows, the last first with `down`; `read(i)` is called behind the i-th one's reading.
+template <typename OUT, bool GROUPED, int RUNS, typename Read>
+__device__ __forceinline__ void store_unit(const Product& p, const Unit& u, const Rows<RUNS>& rows, uint32_t tmem, int q, int set,
+                                           int sets, int lane, bool down, Read read) {
+    const bool pairs = p.unit == GATED;
+    // this thread's output
+    const int n = pairs ? u.n0 / 2 + q * 16 + (lane & 15) : u.n0 + q * 32 + lane;
+    const bool mine = n < p.width;
+    OUT* out = (OUT*)p.out + n;
+    const uint32_t d = tmem + ((uint32_t)(q * 32) << 16);
+#pragma unroll
+    for (int i = 0; i < RUNS; ++i) {
+        const int c0 = ((down ? RUNS - 1 - i : i) * sets + set) * 16, there = u.rows - c0;
+        if (there <= 0) {
+            read(i);
+            continue;
+        }
+        const int to = down ? rows.to[RUNS - 1 - i] : rows.to[i];
+        uint32_t v[16];
+        tmem_ld16(d + c0, v);
+        tmem_ld_wait();
+        read(i);
+        if (GROUPED && p.scale) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x)
+                v[x] = __float_as_uint(__uint_as_float(v[x]) *
+                                       __shfl_sync(0xffffffffu, down ? rows.share[RUNS - 1 - i] : rows.share[i], x));
+        }
+        if (pairs) {
+            // lanes 0..15 hold the gate's sums of 16 rows, lanes 16..31 up's of the same outputs: the former take the
+            // first eight rows, the latter the others
+            const bool upper = lane >= 16;
+            OUT* at = out + (size_t)(u.row0 + c0 + (upper ? 8 : 0)) * p.width;
+            float val[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                const uint32_t others = upper ? v[x] : v[x + 8];
+                const float got = __shfl_xor_sync(0xffffffffu, __uint_as_float(others), 16);
+                const float own = __uint_as_float(upper ? v[x + 8] : v[x]);
+                val[x] = unit_of_sums<OUT>(upper ? got : own, upper ? own : got, p.alpha, p.limit);
+            }
+#pragma unroll
+            for (int x = 0; x < 8; ++x, at += p.width)
+                if (mine && (upper ? x + 8 : x) < there) Elem<OUT>::store(at, val[x]);
+        } else if (GROUPED && p.unit == DOWN) {
+#pragma unroll
+            for (int x = 0; x < 16; ++x) {
+                const int s = __shfl_sync(0xffffffffu, to, x);
+                if (mine && x < there) Elem<OUT>::store(out + (size_t)s * p.width, __uint_as_float(v[x]));
+            }
+        } else {
+            const bool square = p.unit == RELU2;
+            OUT* at = out + (size_t)(u.row0 + c0) * p.width;
+#pragma unroll
+            for (int x = 0; x < 16; ++x, at += p.width) {
+                float val = __uint_as_float(v[x]);
+                if (square) val = fmaxf(val, 0.f) * fmaxf(val, 0.f);
+                if (mine && x < there) Elem<OUT>::store(at, val);
+            }
+        }
+    }
 }
 
 // The whole of a block's work: see mx4_gemm.cu.
@@ -155,34 +340,7 @@ __device__ __forceinline__ void product_block(const Product& p, const CUtensorMa
         chain_release();                 // (not before: see there)
     }
     chain_wait();
-    if (GROUPED && warp == 0) {
-        // start[e]: row tiles of the experts before e.  A lane takes neighbouring experts, whose loads are under way
-        // together.
-        const int per = (p.n_experts + 31) / 32, e0 = min(lane * per, p.n_experts), e1 = min(e0 + per, p.n_experts);
-        int sum = 0, at = e0 < e1 ? p.offsets[e0] : 0;
-#pragma unroll 8
-        for (int e = e0; e < e1; ++e) {
-            const int next = p.offsets[e + 1];
-            sum += (next - at + NT - 1) / NT;
-            at = next;
-        }
-        int before = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, before, o);
-            if (lane >= o) before += x;
-        }
-        if (lane == 31) start[p.n_experts] = before;
-        before -= sum;
-        at = e0 < e1 ? p.offsets[e0] : 0;
-#pragma unroll 8
-        for (int e = e0; e < e1; ++e) {
-            const int next = p.offsets[e + 1];
-            start[e] = before;
-            before += (next - at + NT - 1) / NT;
-            at = next;
-        }
-    }
+    if (GROUPED && warp == 0) row_tiles<NT>(p, lane, start);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -229,54 +387,40 @@ __device__ __forceinline__ void product_block(const Product& p, const CUtensorMa
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- instructions
-        {
-            int g = 0, it = 0;
-            for (int i = blockIdx.x; i < units && !timed_out; i += gridDim.x, ++it) {
-                const Unit u = unit_of<NT, GROUPED>(p, i, m_tiles, start);
-                const int n = (u.rows + 15) & ~15;
-                const uint32_t idesc0 = idesc_mx4(UMMA_M, n, 0), idesc1 = idesc_mx4(UMMA_M, n, 1);
-                const int acc = it % L::ACCS;
-                if (!mbar_wait_warp(acc_empty(acc), ((it / L::ACCS) & 1) ^ 1)) {
+        const uint64_t first = umma_desc(base), first_sf = atom_desc(base + L::SF_A);
+        int it = 0, slot = 0, phase = 0;
+        for (int i = blockIdx.x; i < units && !timed_out; i += gridDim.x, ++it) {
+            const Unit u = unit_of<NT, GROUPED>(p, i, m_tiles, start);
+            const int n = (u.rows + 15) & ~15;
+            const uint32_t idesc0 = idesc_mx4(UMMA_M, n, 0), idesc1 = idesc_mx4(UMMA_M, n, 1);
+            const int acc = it % L::ACCS;
+            if (!mbar_wait_warp(acc_empty(acc), ((it / L::ACCS) & 1) ^ 1)) {
+                timed_out = true;
+                break;
+            }
+            const uint32_t d = tmem_base + acc * NT;
+            int left = p.K;
+            for (int kb = 0; kb < kblocks; ++kb, left -= BK) {
+                if (!mbar_wait_warp(full(slot), phase)) {
                     timed_out = true;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t d = tmem_base + acc * NT;
-                for (int kb = 0; kb < kblocks; ++kb, ++g) {
-                    const int slot = g % L::STAGES;
-                    if (!mbar_wait_warp(full(slot), (g / L::STAGES) & 1)) {
-                        timed_out = true;
-                        break;
-                    }
-                    tc_fence_after();
-                    const uint32_t a = base + slot * L::STAGE, b = a + L::A_BYTES;
-                    // (every stage has its own columns: a copy into them comes behind the barrier that says that
-                    // the instructions which read them last are done)
-                    const uint32_t sf = tmem_base + L::SF_AT + slot * L::SF_STAGE_COLS;
-                    const uint32_t sf_b = sf + SF_COLS;
-                    const int steps = min(4, (p.K - kb * BK + 63) / 64);
-                    if (elect_one()) {
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) copy_atom(sf + x * 4, atom_desc(a + L::SF_A + x * ATOM));
-#pragma unroll
-                        for (int j = 0; j < L::B_TILES; ++j)
-#pragma unroll
-                            for (int x = 0; x < 2; ++x)
-                                copy_atom(sf_b + (x * L::B_TILES + j) * 4,
-                                          atom_desc(a + L::SF_B + j * SF_STAGE + x * ATOM));
-#pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            if (kk < steps)
-                                umma_mx4(d, umma_desc(a + kk * 32), umma_desc(b + kk * 32), kk & 1 ? idesc1 : idesc0,
-                                         sf + (kk >> 1) * 4, sf_b + (kk >> 1) * (L::B_TILES * 4) + u.sf_row / 32,
-                                         (kb | kk) ? 1u : 0u);
-                        umma_commit(empty(slot));
-                    }
-                    __syncwarp();
+                // (every stage has its own columns: a copy into them comes behind the barrier that says that the
+                // instructions which read them last are done)
+                const uint32_t sf = tmem_base + L::SF_AT + slot * L::SF_STAGE_COLS;
+                const uint64_t a = first + slot * (L::STAGE >> 4), scales = first_sf + slot * (L::STAGE >> 4);
+                if (elect_one()) {
+                    copy_scales<false, L::B_TILES>(sf, sf + SF_COLS, scales, scales + (SF_STAGE >> 4));
+                    multiply_stage<false, L::B_TILES>(d, a, a + (L::A_BYTES >> 4), idesc0, idesc1, sf, sf + SF_COLS + u.sf_row / 32,
+                                                      kb > 0, left >= BK ? 4 : (left + 63) / 64);
+                    umma_commit(empty(slot));
                 }
-                if (elect_one()) umma_commit(acc_full(acc));
                 __syncwarp();
+                if (++slot == L::STAGES) slot = 0, phase ^= 1;
             }
+            if (elect_one()) umma_commit(acc_full(acc));
+            __syncwarp();
         }
     } else {
         // -------------------------------------------------------------------- epilogue
@@ -285,58 +429,17 @@ __device__ __forceinline__ void product_block(const Product& p, const CUtensorMa
         for (int i = blockIdx.x; i < units; i += gridDim.x, ++it) {
             const Unit u = unit_of<NT, GROUPED>(p, i, m_tiles, start);
             const int acc = it % L::ACCS;
-            const bool pairs = p.unit == GATED;
-            // this thread's output
-            const int n = pairs ? u.n0 / 2 + q * 16 + (lane & 15) : u.n0 + q * 32 + lane;
-            const bool mine = n < p.width;
+            constexpr int RUNS = NT / 16 / 2;
+            const Rows<RUNS> r = rows_of<GROUPED, RUNS>(p, u, half, 2, lane);
             if (!mbar_wait_warp(acc_full(acc), (it / L::ACCS) & 1)) {
                 timed_out = true;
                 break;
             }
             tc_fence_after();
-            const uint32_t d = tmem_base + acc * NT + ((uint32_t)(q * 32) << 16);
-#pragma unroll 1
-            for (int c0 = half * 16; c0 < u.rows; c0 += 32) {
-                uint32_t v[16];
-                tmem_ld16(d + c0, v);
-                // where row c0 + lane goes, and the weight of its slot
-                int to = u.row0 + c0 + lane;
-                float share = 1.f;
-                if (GROUPED && lane < 16 && c0 + lane < u.rows && (p.unit == DOWN || p.scale)) {
-                    const int s = p.order[to];
-                    if (p.scale) share = p.weight[s];
-                    if (p.unit == DOWN) to = s;
-                }
-                tmem_ld_wait();
-                if (GROUPED && p.scale) {
-#pragma unroll
-                    for (int x = 0; x < 16; ++x)
-                        v[x] = __float_as_uint(__uint_as_float(v[x]) * __shfl_sync(0xffffffffu, share, x));
-                }
-                if (pairs) {
-                    // lanes 0..15 hold the gate's sums of 16 rows, lanes 16..31 up's of the same outputs: the former take the
-                    // first eight rows, the latter the others
-                    const bool upper = lane >= 16;
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        const uint32_t mine_v = upper ? v[x + 8] : v[x], others = upper ? v[x] : v[x + 8];
-                        const float got = __shfl_xor_sync(0xffffffffu, __uint_as_float(others), 16);
-                        const float own = __uint_as_float(mine_v);
-                        const float val = mls_experts::gated_unit(upper ? got : own, upper ? own : got, p.alpha, p.limit);
-                        const int row = upper ? x + 8 : x;
-                        const int s = __shfl_sync(0xffffffffu, to, row);
-                        if (mine && c0 + row < u.rows) store_from_float(p.out, (size_t)s * p.width + n, p.out_type, val);
-                    }
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 16; ++x) {
-                        const int s = __shfl_sync(0xffffffffu, to, x);
-                        float val = __uint_as_float(v[x]);
-                        if (p.unit == RELU2) val = fmaxf(val, 0.f) * fmaxf(val, 0.f);
-                        if (mine && c0 + x < u.rows) store_from_float(p.out, (size_t)s * p.width + n, p.out_type, val);
-                    }
-                }
-            }
+            const uint32_t d = tmem_base + acc * NT;
+            auto read = [](int) {};
+            if (p.out_type == MLS_BF16) store_unit<__nv_bfloat16, GROUPED, RUNS>(p, u, r, d, q, half, 2, lane, false, read);
+            else store_unit<float, GROUPED, RUNS>(p, u, r, d, q, half, 2, lane, false, read);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty(acc));

@@ -1,0 +1,325 @@
+// The product of many rows by pairs of blocks: two neighbouring SMs work on one tile of 256 of one operand's rows (the M side)
+// by up to NT of the other's (the N side).
+//
+// At four bits a value an instruction is done with its operands in a third of the time in which L2 brings them to a lone block,
+// whose 128 x 192 tile asks for 43 KB for every 256 of K.  Here a block brings in its 128 rows of the M side and half of the N
+// side's (31 KB for 128 x 192, 35 for 128 x 256), and the instruction, issued by the first block of the pair, takes both
+// halves.  Each block holds the scales of its own M rows and of all N rows.
+//
+// One matrix: the batch's rows are the M side, the weights the N side.  A thread of the epilogue then holds neighbouring
+// outputs of one row, gate and up of the same output among them, and stores whole sectors of 32 bytes.  (With the weights on
+// the M side a warp's stores are 64 bytes of a row each: 2,048 rows x 28,672 x 4,096 with SwiGLU took 213 us, of which the
+// epilogue was 110.)
+// Routed: the weights are the M side, an expert's rows the N side, rounded up to 32 only: experts of a prompt have from ten to
+// some hundreds of rows, of which tiles of 256 would waste half the instructions.
+//
+// Tensor memory: ACC_COLS columns of accumulators, every second one from the first column on, the others up to the last, so that
+// two that fit beside one another overlap: the epilogue of one lies under the instructions of the next.  NT = 192 always fits;
+// one of 256 asks for fewer bytes, but waits until half of the one before it has been read: the half that it takes, which is
+// read first.  Behind them the scales of the last SF_SLOTS stages.
+//
+// Hand-overs inside the pair, as in the bfloat16 product: full[s] (first block) counts both blocks' copies; empty[s] and acc_full[a]
+// arrive on both blocks' barriers; acc_free[a] and acc_empty[a] (first block) take the arrivals of both blocks' epilogue warps,
+// when they have read the half of an accumulator that the next may take, and all of it.  No load is multicast.  These kernels are launched plainly: chained behind a long quantisation of rows a run under a profiler did not end.
+#pragma once
+#include "mx4_gemm.h"
+
+namespace mls_mx4 {
+
+// A box of a 3-D tensor map, from either block of a pair, that completes on the first one's barrier.
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .b32 rbar;\n\t"
+        "mapa.shared::cluster.u32 rbar, %2, 0;\n\t"
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [rbar];\n\t}"
+        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+
+template <int NT_, bool GROUPED>
+struct PairPlan {
+    static constexpr int NT = NT_, MT = 2 * UMMA_M;
+    static constexpr int BOX = GROUPED ? 64 : NT / 2;              // N rows of a copy
+    static constexpr int A_BYTES = UMMA_M * CODE_ROW, B_BYTES = NT / 2 * CODE_ROW;
+    static constexpr int SF_A = A_BYTES + B_BYTES, SF_B = SF_A + SF_STAGE;
+    static constexpr int STAGE = SF_B + 2 * SF_STAGE;
+    static constexpr int STAGES = (220 * 1024) / STAGE;
+    static constexpr int SF_SLOT_COLS = 3 * SF_COLS;
+    static constexpr int ACC_COLS = 384;
+    static constexpr int FIT = (512 - ACC_COLS) / SF_SLOT_COLS;
+    static constexpr int SF_SLOTS = FIT < STAGES ? FIT : STAGES;
+    static constexpr int SETS = GROUPED ? 4 : NT / 64;             // of four epilogue warps
+    static constexpr int THREADS = 64 + 128 * SETS;
+    static constexpr int BARS = STAGES * STAGE;                    // full, empty [STAGES]; acc_full, acc_free, acc_empty [2]
+    static constexpr int TMEM_SLOT = BARS + 8 * (2 * STAGES + 6);
+    static constexpr int TABLE = TMEM_SLOT + 16;
+    static constexpr int FIXED = TABLE + 1024;
+    static_assert(ACC_COLS + SF_SLOTS * SF_SLOT_COLS <= 512 && STAGE % 1024 == 0 && ACC_COLS >= NT &&
+                  FIXED + 4 * (TABLE_EXPERTS + 1) <= 227 * 1024, "tile");
+};
+
+// 32 bytes of a row at a 32-byte place: whole sectors, where a warp's lanes store to 32 rows.
+__device__ __forceinline__ void store32(void* at, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};\n"
+                 ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+// COUNT neighbouring outputs of a row, `there` of which exist; vec: the row's runs start at 32-byte places.
+template <typename OUT, int COUNT>
+__device__ __forceinline__ void store_run(OUT* out, const float (&v)[COUNT], int there, bool vec) {
+    constexpr int PER = 32 / sizeof(OUT);
+    if (vec && there >= COUNT) {
+#pragma unroll
+        for (int i = 0; i < COUNT / PER; ++i) {
+            uint32_t w[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (sizeof(OUT) == 2) {
+                    const __nv_bfloat162 h = __floats2bfloat162_rn(v[PER * i + 2 * j], v[PER * i + 2 * j + 1]);
+                    memcpy(&w[j], &h, 4);
+                } else {
+                    w[j] = __float_as_uint(v[PER * i + j]);
+                }
+            }
+            store32(out + PER * i, w);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i)
+            if (i < there) Elem<OUT>::store(out + i, v[i]);
+    }
+}
+
+// A warp's runs of 32 columns of the accumulator, for its 32 rows: this thread's goes to row `to`.  The set's runs lie `step`
+// columns apart, in the order in which they are to be read; `read(i)` is called behind the i-th one's reading.
+template <typename OUT, int RUNS, typename Read>
+__device__ __forceinline__ void store_rows(const Product& p, uint32_t d, int set, int sets, bool down, int columns, int n0,
+                                           bool any, bool mine, int to, bool vec, Read read) {
+    OUT* row = (OUT*)p.out + (size_t)to * p.width;
+    const bool pairs = p.unit == GATED, square = p.unit == RELU2;
+#pragma unroll 1
+    for (int i = 0; i < RUNS; ++i) {
+        const int c0 = ((down ? RUNS - 1 - i : i) * sets + set) * 32;
+        if (!any || c0 >= columns) {                 // (nothing to read)
+            read(i);
+            continue;
+        }
+        uint32_t x[16], y[16];
+        tmem_ld16(d + c0, x);
+        tmem_ld16(d + c0 + 16, y);
+        tmem_ld_wait();
+        read(i);
+        if (pairs) {
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                v[j] = unit_of_sums<OUT>(__uint_as_float(x[j]), __uint_as_float(y[j]), p.alpha, p.limit);
+            }
+            const int col = (n0 + c0) / 2;
+            if (mine) store_run<OUT>(row + col, v, p.width - col, vec);
+        } else {
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                v[j] = __uint_as_float(j < 16 ? x[j & 15] : y[j & 15]);
+                if (square) v[j] = fmaxf(v[j], 0.f) * fmaxf(v[j], 0.f);
+            }
+            const int col = n0 + c0;
+            if (mine) store_run<OUT>(row + col, v, p.width - col, vec);
+        }
+    }
+}
+
+// m_map, n_map: codes of the operands; sf_m_map, sf_n_map: their scales.
+template <int NT_, bool GROUPED>
+__device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* m_map, const CUtensorMap* n_map,
+                                           const CUtensorMap* sf_m_map, const CUtensorMap* sf_n_map) {
+    using L = PairPlan<NT_, GROUPED>;
+    constexpr int ROW_TILE = GROUPED ? L::NT : L::MT, W_TILE = GROUPED ? L::MT : L::NT;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_u32(smem_raw);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    uint8_t* gbase = smem_raw + (base - raw);
+    auto full = [&](int s) { return base + L::BARS + 8u * s; };
+    auto empty = [&](int s) { return base + L::BARS + 8u * (L::STAGES + s); };
+    auto acc_full = [&](int a) { return base + L::BARS + 8u * (2 * L::STAGES + a); };
+    auto acc_free = [&](int a) { return base + L::BARS + 8u * (2 * L::STAGES + 2 + a); };
+    auto acc_empty = [&](int a) { return base + L::BARS + 8u * (2 * L::STAGES + 4 + a); };
+    volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(gbase + L::TMEM_SLOT);
+    int* start = reinterpret_cast<int*>(gbase + L::TABLE);
+
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();                          // 0: issues the instructions
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < L::STAGES; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(acc_full(a), 1);
+            mbar_init(acc_free(a), 2 * 4 * L::SETS);
+            mbar_init(acc_empty(a), 2 * 4 * L::SETS);
+        }
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        tmem_alloc_pair(smem_u32(const_cast<uint32_t*>(tmem_slot)), 512);
+        chain_release();                 // (not before: see there)
+    }
+    chain_wait();
+    if (GROUPED && warp == 0) row_tiles<ROW_TILE>(p, lane, start);
+    tc_fence_before();
+    __syncwarp();
+    cluster_sync_all();                  // both blocks' barriers, tables and tensor memory are ready
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+    const int w_tiles = (p.N + W_TILE - 1) / W_TILE, sf_tiles = (p.N + TILE_ROWS - 1) / TILE_ROWS;
+    const int units = (GROUPED ? start[p.n_experts] : (p.M + ROW_TILE - 1) / ROW_TILE) * w_tiles;
+    const int kblocks = (p.K + BK - 1) / BK;
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    bool timed_out = false;
+    // the accumulator's columns, up to a multiple of 32 (a half of the N rows comes from each block), and where they are
+    auto columns = [&](const Unit& u) { return ((GROUPED ? u.rows : min(L::NT, p.N - u.n0)) + 31) & ~31; };
+    auto place = [&](const Unit& u, int it) { return it & 1 ? L::ACC_COLS - columns(u) : 0; };
+
+    if (warp == 0) {
+        // ----------------------------------------------------------------- TMA producer
+        if (lane == 0) {
+            int g = 0;
+            for (int i = first; i < units && !timed_out; i += step) {
+                const Unit u = unit_of<ROW_TILE, GROUPED, W_TILE>(p, i, w_tiles, start);
+                const int half = columns(u) / 2, boxes = GROUPED ? (half + L::BOX - 1) / L::BOX : 1;
+                const uint32_t bytes = 2 * (L::A_BYTES + boxes * (L::BOX * CODE_ROW) + 3 * SF_STAGE);
+                const int w_row = u.e * p.N + u.n0, sf_w = u.e * sf_tiles + u.n0 / TILE_ROWS;
+                const int m_row = (GROUPED ? w_row : u.row0) + (int)rank * UMMA_M;
+                const int n_row = (GROUPED ? u.row0 : w_row) + (int)rank * half;
+                const int sf_m = (GROUPED ? sf_w : u.sf_tile) + (int)rank, sf_n = GROUPED ? u.sf_tile : sf_w;
+                for (int kb = 0; kb < kblocks; ++kb, ++g) {
+                    const int slot = g % L::STAGES;
+                    if (!mbar_wait(empty(slot), ((g / L::STAGES) & 1) ^ 1)) {
+                        timed_out = true;
+                        break;
+                    }
+                    const uint32_t a = base + slot * L::STAGE, b = a + L::A_BYTES, bar = full(slot);
+                    // both blocks' copies of the stage complete on the first one's barrier
+                    if (rank == 0) mbar_arrive_expect_tx(bar, bytes);
+                    tma_load_2d_pair(a, m_map, kb * CODE_ROW, m_row, bar);
+                    for (int x = 0; x < boxes; ++x)
+                        tma_load_2d_pair(b + x * (L::BOX * CODE_ROW), n_map, kb * CODE_ROW, n_row + x * L::BOX, bar);
+                    tma_load_3d_pair(a + L::SF_A, sf_m_map, 0, kb, sf_m, bar);
+                    tma_load_3d_pair(a + L::SF_B, sf_n_map, 0, kb, sf_n, bar);
+                }
+            }
+            // the copies under way land before the pair's shared memory goes away (the first block's barriers count both
+            // blocks' bytes, and both blocks meet once more)
+            if (rank == 0)
+                for (int j = g > L::STAGES ? g - L::STAGES : 0; j < g; ++j)
+                    if (!mbar_wait_cluster(full(j % L::STAGES), (j / L::STAGES) & 1)) timed_out = true;
+        }
+    } else if (warp == 1) {
+        if (rank == 0) {
+            // ---------------------------------------------------- instructions, for the pair
+            // What a stage costs this warp beside the instructions bounds tiles of few columns: 0.39 us a stage with the
+            // places of slots divided out anew and waits one by one, XXX now; the instructions of 256 columns take 0.33.
+            constexpr bool FEWER = L::SF_SLOTS < L::STAGES;
+            const uint64_t first_a = umma_desc(base), first_sf = atom_desc(base + L::SF_A);
+            int it = 0, columns_before = 0, slot = 0, phase = 0;
+            int sf_slot = 0, old = L::STAGES - L::SF_SLOTS, old_phase = 1;      // (the phase before the first is over)
+            for (int i = first; i < units && !timed_out; i += step, ++it) {
+                const Unit u = unit_of<ROW_TILE, GROUPED, W_TILE>(p, i, w_tiles, start);
+                const int n = columns(u), acc = it & 1;
+                const uint32_t idesc0 = idesc_mx4(2 * UMMA_M, n, 0), idesc1 = idesc_mx4(2 * UMMA_M, n, 1);
+                // the accumulator before the last has been read, and of the last the columns that this one may take, where
+                // it does not fit beside it
+                if (!mbar_wait_cluster_warp(acc_empty(acc), ((it >> 1) & 1) ^ 1) ||
+                    (columns_before + n > L::ACC_COLS &&
+                     !mbar_wait_cluster_warp(acc_free(acc ^ 1), ((it - 1) >> 1) & 1))) {
+                    timed_out = true;
+                    break;
+                }
+                columns_before = n;
+                const uint32_t d = tmem_base + place(u, it), shift = (GROUPED ? u.sf_row : u.n0 % TILE_ROWS) / 32;
+                int left = p.K;
+                for (int kb = 0; kb < kblocks; ++kb, left -= BK) {
+                    // the stage is there, and the instructions that read its scales' columns last are done: both asked at
+                    // once, one by one only where one of them is not
+                    bool ready = mbar_try_wait_cluster(full(slot), phase);
+                    if (FEWER) ready &= mbar_try_wait(empty(old), old_phase);
+                    if (!__all_sync(0xffffffffu, ready) &&
+                        (!mbar_wait_cluster_warp(full(slot), phase) || (FEWER && !mbar_wait_warp(empty(old), old_phase)))) {
+                        timed_out = true;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t sf = tmem_base + L::ACC_COLS + sf_slot * L::SF_SLOT_COLS;
+                    const uint64_t a = first_a + slot * (L::STAGE >> 4), scales = first_sf + slot * (L::STAGE >> 4);
+                    if (elect_one()) {
+                        copy_scales<true, 2>(sf, sf + SF_COLS, scales, scales + (SF_STAGE >> 4));
+                        multiply_stage<true, 2>(d, a, a + (L::A_BYTES >> 4), idesc0, idesc1, sf, sf + SF_COLS + shift, kb > 0,
+                                                left >= BK ? 4 : (left + 63) / 64);
+                        umma_commit_pair(empty(slot), 3);          // both blocks' stage is free
+                    }
+                    __syncwarp();
+                    if (++slot == L::STAGES) slot = 0, phase ^= 1;
+                    if (++sf_slot == L::SF_SLOTS) sf_slot = 0;
+                    if (++old == L::STAGES) old = 0, old_phase ^= 1;
+                }
+                if (elect_one()) umma_commit_pair(acc_full(acc), 3);   // both blocks' accumulator is complete
+                __syncwarp();
+            }
+        }
+    } else {
+        // -------------------------------------------------------------------- epilogue
+        const int q = warp & 3, set = (warp - 2) >> 2;
+        // runs of 16 (routed) or 32 columns a set: two or more, the first half of them in the columns that the next may take
+        constexpr int RUNS = L::NT / (GROUPED ? 16 : 32) / L::SETS, FREE_AT = L::NT == 256 ? RUNS / 2 - 1 : RUNS - 1;
+        const bool vec = p.width % (p.out_type == MLS_BF16 ? 16 : 8) == 0 && reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
+        auto arrive = [&](uint32_t bar) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (rank == 0) mbar_arrive(bar);
+                else mbar_arrive_remote(bar, 0);
+            }
+        };
+        int it = 0;
+        for (int i = first; i < units; i += step, ++it) {
+            Unit u = unit_of<ROW_TILE, GROUPED, W_TILE>(p, i, w_tiles, start);
+            const int acc = it & 1;
+            // (the columns in the middle first: an accumulator at the end begins there, one at the start ends there)
+            const bool down = acc == 0;
+            const uint32_t d = tmem_base + place(u, it);
+            auto read = [&](int run) {
+                if (run == FREE_AT) arrive(acc_free(acc));
+                if (run == RUNS - 1) arrive(acc_empty(acc));
+            };
+            Rows<RUNS> r;
+            if (GROUPED) r = rows_of<GROUPED, RUNS>(p, u, set, L::SETS, lane);
+            if (!mbar_wait_warp(acc_full(acc), (it >> 1) & 1)) {
+                timed_out = true;
+                break;
+            }
+            tc_fence_after();
+            if constexpr (GROUPED) {
+                u.n0 += (int)rank * UMMA_M;
+                if (p.out_type == MLS_BF16) store_unit<__nv_bfloat16, GROUPED, RUNS>(p, u, r, d, q, set, L::SETS, lane, down, read);
+                else store_unit<float, GROUPED, RUNS>(p, u, r, d, q, set, L::SETS, lane, down, read);
+            } else {
+                const int row = (int)rank * UMMA_M + q * 32 + lane;
+                const uint32_t at = d + ((uint32_t)(q * 32) << 16);
+                const bool any = (int)rank * UMMA_M + q * 32 < u.rows, mine = row < u.rows;
+                if (p.out_type == MLS_BF16)
+                    store_rows<__nv_bfloat16, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, mine, u.row0 + row, vec, read);
+                else
+                    store_rows<float, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, mine, u.row0 + row, vec, read);
+            }
+        }
+    }
+    if (timed_out && p.status) atomicOr(p.status, MLS_STATUS_TIMEOUT);
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync_all();                  // nobody of the pair touches tensor memory any more
+    if (warp == 1) tmem_dealloc_pair(tmem_base, 512);
+}
+}  // namespace mls_mx4

@@ -217,6 +217,7 @@ class Ops:
         self._sample = _decl(core, "mls_sample", [_P, _P, _P, _P, _I, _I, _P, _P])
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._status_at = self.status.data_ptr()
+        self._mx4_captured, self._mx4_kept = None, []
         self._attention_libs: dict = {}
         self._attention_lib_handles: dict = {}
         self._split_ctas_per_sm: dict = {}       # head size -> CTAs of the split kernel an SM holds
@@ -993,7 +994,7 @@ class Ops:
                                     [_I, _P, _I, _LL, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F,
                                      _P, _P]),
                    "expert_product": _decl(lib, "mls_mx4_expert_product",
-                                           [_I, _P, _I, _LL, _I, _I, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I,
+                                           [_I, _P, _I, _LL, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I,
                                             _P, _P, _P, _P, _I, _F, _F, _P, _P])}
         elif name == "shortconv":
             fns = {"qk": _decl(lib, "mls_qk_conv_norm_rope_store",
@@ -1463,6 +1464,7 @@ class Ops:
 
     # ------------------------------------------------- 4-bit microscaled rows and weights
     MX4_MOST_K = 1 << 20
+    MX4_ONCE = 1 << 16       # slots x steps of 256 of K from which on tokens are quantised once
     MX4_FUSED_TASKS = 64     # 256 values of a row each: with so many a block the product quantises its rows itself
 
     def _mx4_here(self, what: str, *tensors) -> None:
@@ -1551,12 +1553,20 @@ class Ops:
             held.settled = True
         return held
 
-    def _mx4_scratch(self, m: int, k: int, tiles: int) -> tuple:
-        """Addresses of the codes and scales of a product's rows in scratch memory."""
-        scales = tiles * Mx4.tile_bytes(k)
-        held = self.scratch("mx4_rows", (m * Mx4.pitch(k) + scales) // 4)
-        at = held.data_ptr()
-        return at + scales, at
+    def _mx4_scratch(self, m: int, k: int, tiles: int, tokens: int = 0) -> tuple:
+        """Addresses of the codes and scales of a product's rows in scratch memory, and of those of the tokens that they are
+        gathered from."""
+        pitch, tile = Mx4.pitch(k), Mx4.tile_bytes(k)
+        token_tiles = (tokens + 127) // 128
+        held = self.scratch("mx4_rows", ((m + tokens) * pitch + (tiles + token_tiles) * tile) // 4)
+        if torch.cuda.is_current_stream_capturing() and held is not self._mx4_captured:
+            # a graph goes on writing there: the memory stays, whatever later products need
+            self._mx4_captured = held
+            self._mx4_kept.append(held)
+        sf = held.data_ptr()
+        sf_tokens = sf + tiles * tile
+        codes = sf_tokens + token_tiles * tile
+        return codes, sf, codes + m * pitch, sf_tokens
 
     def _product_mx4(self, unit: int, a, w: Mx4, out, what: str, alpha=1.0, limit=0.0) -> None:
         if w.__class__ is not Mx4 or w.lead or w.gate_up != (unit == 1):
@@ -1584,7 +1594,7 @@ class Ops:
             code, ld, rows = self._mx4_type(a, what), self._mx4_ld(a, k, what), a.data_ptr()
             fused = 0 < few <= 12 and m <= 16 and m * few <= self.MX4_FUSED_TASKS
             if not fused:
-                codes, scales = self._mx4_scratch(m, k, (m + 127) // 128)
+                codes, scales, _, _ = self._mx4_scratch(m, k, (m + 127) // 128)
                 self.launches += 1
         self.launches += 1
         rc = self._part_lib("mx4")["product"](unit, rows, code, ld, codes, scales, w.codes_at, w.scales_at, out.data_ptr(),
@@ -1630,10 +1640,13 @@ class Ops:
         self._mx4_here(what, rows, w.data, out, order, idx, offsets, weight)
         if slots == 0 or n_experts == 0 or n == 0:
             return
-        codes, scales = self._mx4_scratch(slots, k, slots // 128 + n_experts + 1)
-        self.launches += 1 - (-n_experts // 1024)
+        # (many slots: every token is quantised once and copied to its slots; 12,288 slots of 2,048 tokens x 4,096 in 12 us
+        # where they took 27 one by one)
+        tokens = shape[0] if unit and top > 1 and slots * -(-k // 256) >= self.MX4_ONCE else 0
+        codes, scales, t_codes, t_scales = self._mx4_scratch(slots, k, slots // 128 + n_experts + 1, tokens)
+        self.launches += (2 if tokens else 1) - (-n_experts // 1024)
         rc = self._part_lib("mx4")["expert_product"](
-            unit, rows.data_ptr(), code, ld, top, unit != 0, codes, scales, w.codes_at, w.scales_at, out.data_ptr(), out_type,
+            unit, rows.data_ptr(), code, ld, top, unit != 0, tokens, t_codes, t_scales, codes, scales, w.codes_at, w.scales_at, out.data_ptr(), out_type,
             slots, n_experts, n, k, order.data_ptr(), idx.data_ptr(), offsets.data_ptr(), weight.data_ptr(), scale, alpha,
             limit, self._status_at, self._stream())
         if rc:

@@ -57,8 +57,8 @@ MODULES = {
     "mx4": ["mx4.cu", "mx4_gemm.cu"],
 }
 
-# headers of other modules' sources that a module's sources include
-SHARED_HEADERS = {"mx4": ["experts.h"]}
+# headers that a module's sources include beside their own
+SHARED_HEADERS = {"mx4": ["experts.h", "mx4_few.h", "mx4_pair.h"]}
 
 
 def all_modules(head_sizes=()) -> list:

@@ -175,7 +175,7 @@ EXPERTS = [  # tokens, experts, outputs without weights, top, d, f, spread
     (33, 5, 0, 2, 65, 131, "one"), (65, 9, 0, 2, 257, 136, "one"), (40, 2, 0, 1, 200, 129, "even"),
     (129, 3, 0, 2, 64, 96, "one"), (127, 2, 0, 2, 320, 264, "even"), (257, 3, 1, 2, 128, 72, "one"),
     (600, 4, 0, 1, 64, 130, "even"), (515, 2, 0, 1, 256, 384, "one"), (70, 300, 0, 3, 64, 32, "even"),
-    (30, 1500, 3, 2, 40, 24, "even")]
+    (30, 1500, 3, 2, 40, 24, "even"), (2100, 5, 1, 3, 2900, 72, "one")]
 
 
 @pytest.mark.parametrize("t, experts, identity, top, d, f, spread", EXPERTS)
