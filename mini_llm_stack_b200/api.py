@@ -51,6 +51,7 @@ def cmd_chat(args) -> int:
                          max_batch=args.max_batch,
                          max_tokens_per_step=args.max_tokens_per_step,
                          chunk_size=args.chunk_size, dtype=args.dtype, device=args.device,
+                         ffn_weights=args.ffn_weights,
                          kv_dtype=args.kv_dtype, seed=args.sample_seed)
     if args.model:
         llm = LLM.from_folder(args.model, options=opts)
@@ -109,6 +110,8 @@ def main(argv=None) -> int:
     c.add_argument("--dtype", choices=["bfloat16", "float32"], default=None)
     c.add_argument("--kv-dtype", choices=["bfloat16", "float32"], default=None,
                    help="must equal the run's dtype (the cache is kept in it)")
+    c.add_argument("--ffn-weights", choices=["mxfp4"], default=None,
+                   help="hold the feed-forward weights as 4-bit microscaled values (default: as loaded)")
     c.add_argument("--device", default="cuda:0")
     c.add_argument("--num-blocks", type=int, default=512)     # serve/api.py:92
     c.add_argument("--block-size", type=int, default=16)

@@ -8,6 +8,7 @@
 // product takes two at a time).
 #pragma once
 #include "common.cuh"
+#include <atomic>
 #include <cuda_fp16.h>
 #include <string.h>
 
@@ -49,6 +50,35 @@ struct RowMap {
     const int *order, *idx, *offsets;              // sorted slots of a routed step (offsets == nullptr: plain rows)
     int top, n_experts, gather;                    // gather: row p is a copy of row order[p] / top
 };
+// What a C entry does, with an exception's end as an error code.
+template <typename Body>
+static inline int guarded(Body body) {
+    try {
+        return body();
+    } catch (...) {
+        return (int)cudaErrorMemoryAllocation;
+    }
+}
+
+// A kernel's limit of shared memory, set once on every device.
+class SharedLimit {
+public:
+    template <typename Kernel>
+    int set(Kernel kernel, int bytes) {
+        int device = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        if (e != cudaSuccess) return (int)e;
+        const unsigned long long bit = 1ull << (device & 63);
+        if (device < 64 && (done_.load() & bit)) return 0;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess) done_.fetch_or(bit);
+        return (int)e;
+    }
+
+private:
+    std::atomic<unsigned long long> done_{0};
+};
+
 // A launch that starts when the kernels before it have finished.
 template <typename... Params, typename... Args>
 static inline int launch_plain(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,

@@ -99,14 +99,8 @@ bool chained(long long rows, int K) { return rows <= 256 && rows * ((K + 255) / 
 template <int NT, bool GROUPED>
 int launch_nt(const Product& p, const void* rows, const void* W, cudaStream_t stream) {
     using L = Plan<NT>;
-    static bool configured = false;
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(mx4_product_kernel<NT, GROUPED>,
-                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   L::FIXED + 4 * (TABLE_EXPERTS + 1));
-        if (e != cudaSuccess) return (int)e;
-        configured = true;
-    }
+    static SharedLimit limit;
+    if (const int e = limit.set(mx4_product_kernel<NT, GROUPED>, L::FIXED + 4 * (TABLE_EXPERTS + 1))) return e;
     CUtensorMap rows_map, w_map;
     if (!codes_map(rows, p.M, p.K, L::BOX, &rows_map) ||
         !codes_map(W, (long long)p.n_experts * p.N, p.K, UMMA_M, &w_map))
@@ -127,13 +121,8 @@ int launch_nt(const Product& p, const void* rows, const void* W, cudaStream_t st
 template <int NT, bool GROUPED>
 int launch_pair(const Product& p, const void* rows, const void* W, cudaStream_t stream) {
     using L = PairPlan<NT, GROUPED>;
-    static bool configured = false;
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(mx4_pair_kernel<NT, GROUPED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   L::FIXED + 4 * (TABLE_EXPERTS + 1));
-        if (e != cudaSuccess) return (int)e;
-        configured = true;
-    }
+    static SharedLimit limit;
+    if (const int e = limit.set(mx4_pair_kernel<NT, GROUPED>, L::FIXED + 4 * (TABLE_EXPERTS + 1))) return e;
     const long long row_tiles = GROUPED ? p.M / TILE_ROWS + p.all_experts + 1 : (p.M + TILE_ROWS - 1) / TILE_ROWS;
     const long long w_tiles = (long long)p.n_experts * ((p.N + TILE_ROWS - 1) / TILE_ROWS);
     CUtensorMap rows_map, w_map, sf_rows_map, sf_w_map;
@@ -157,47 +146,48 @@ int launch_pair(const Product& p, const void* rows, const void* W, cudaStream_t 
 }
 
 // The ways of many rows, by the tile of a unit of work: 128 weights x 64 or 192 rows on one block, 256 rows x 192 or 256 weights on
-// a pair.  Units are dealt out in rounds of one a block or pair; a round takes so long for every 256 of K, and so long for what
-// its epilogue leaves visible.  The cheapest way is taken.  Measured, us, in the order 64 / 192 / 192 on pairs / 256 on pairs:
-//   256 rows x 14,336, 4,096 outputs       21.4 / 29.1 / 23.5 / 22.7     2,048 rows          125 / 81 / 62 / 45
-//   192 x 4,096, 28,672 gated              29 / 19.5 / 22 / 18.7         384 rows            55 / 34.5 / 34.0 / 36.0
-//   707 x 2,048, 16,384 gated              35 / 22.1 / 19.4 / 20.5       2,048 rows          84 / 48 / 40 / 44
-//   256 x 2,048, 2,048                     5.9 / 9.1 / 8.4 / 9.1         2,048 rows          15.7 / 14.1 / 12.9 / 9.9
+// a pair (routed: 256 weights x 256 rows).  Units are dealt out in rounds of one a block or pair; a round takes so long for every
+// 256 of K, and so long for what its epilogue leaves visible (float32 sums of slots are 200 MB in a long prompt).  The
+// cheapest way is taken.  Measured, us, in the order 64 / 192 / 192 on pairs / 256 on pairs, rows quantised already:
+//   256 rows x 14,336, 4,096 outputs       21.4 / 30.3 / 21.5 / 22.5     2,048 rows          125 / 82 / 54 / 42
+//   128 x 4,096, 28,672 gated              23.4 / 16.0 / 20.1 / 17.1     2,048 rows          266 / 134 / 102 / 95
+//   256 x 2,048, 2,048                     5.9 / 10.0 / 8.0 / 8.6        2,048 rows          15.6 / 15.7 / 11.6 / 9.3
+// and routed, the whole call, 64 / 192 / pairs (8b: 64 experts of 4,096 x 1,408, 6 chosen; 1b: 32 of 2,048 x 1,024, 4 chosen):
+//   8b, gate and up, 16 tokens  44.8 / 47.9 / 51.0, 600  98 / 88 / 92, 2,048  212 / 138 / 131
+//   1b, down, 600 tokens        29.4 / 36.1 / 34.5; 8b, 2,048 tokens  191 / 213 / 186
 template <bool GROUPED>
 int launch(const Product& p, const void* rows, const void* W, cudaStream_t stream) {
-    const double k = (p.K + BK - 1) / BK, gated = p.unit == GATED ? 1 : 0;
-    // (routed: experts of somewhat more than the average number of rows)
+    const double k = (p.K + BK - 1) / BK, gated = p.unit == GATED ? 1 : 0, slots = GROUPED && p.unit == DOWN ? 1 : 0;
+    // (routed: a prompt's experts have very unequal numbers of rows, most of the rows lie in experts of half as many again)
     const long long experts = p.M < p.n_experts ? p.M : p.n_experts;
-    const long long each = GROUPED ? (p.M / experts * 11 + 9) / 10 + 1 : p.M;
+    const long long each = GROUPED ? p.M * 3 / (2 * experts) + 1 : p.M;
     const long long sets = GROUPED ? experts : 1;
-    auto cost = [&](long long row_tile, long long w_tile, int places, double per_k, double rest) {
+    auto rows_in = [&](int tile) { return (double)each / (double)((each + tile - 1) / tile); };
+    auto cost = [&](long long row_tile, long long w_tile, int places, double per_k, double rest, double start) {
         const long long units = sets * ((each + row_tile - 1) / row_tile) * ((p.N + w_tile - 1) / w_tile);
-        return (double)((units + places - 1) / places) * (k * per_k + rest);
+        return start + (double)((units + places - 1) / places) * (k * per_k + rest);
     };
     const int blocks = sm_count(), pairs = blocks / 2;
-    const double t[4] = {cost(64, 128, blocks, 0.335, 0.45),
-                         cost(192, 128, blocks, 0.30 + 0.00094 * (double)(each < 192 ? each : 192), 0.8),
-                         GROUPED ? 1e30 : cost(256, 192, pairs, 0.40, 0.3),
-                         cost(256, 256, pairs, 0.375, 1.3 + 1.2 * gated)};
+    const double of_192 = 0.30 + 0.00094 * rows_in(192);
+    const double t[4] = {cost(64, 128, blocks, 0.335, 0.45, 0), cost(192, 128, blocks, of_192 > 0.345 ? of_192 : 0.345,
+                                                                     0.9 + 2.5 * slots, 0),
+                         GROUPED ? 1e30 : cost(256, 192, pairs, 0.355, 0.5 + 0.8 * gated, 1),
+                         GROUPED ? cost(256, 256, pairs, 0.30 + 0.0004 * rows_in(256), 0.9 + 0.6 * gated + 3 * slots, 2)
+                                 : cost(256, 256, pairs, 0.365, 0.9 + 0.6 * gated, 1)};
     int best = 0;
     for (int way = 1; way < 4; ++way)
         if (t[way] < t[best]) best = way;
     return best == 0   ? launch_nt<64, GROUPED>(p, rows, W, stream)
            : best == 1 ? launch_nt<192, GROUPED>(p, rows, W, stream)
-           : best == 2 ? launch_pair<(GROUPED ? 256 : 192), GROUPED>(p, rows, W, stream)
-                       : launch_pair<256, GROUPED>(p, rows, W, stream);
+           : best == 3 || GROUPED ? launch_pair<256, GROUPED>(p, rows, W, stream)
+                                  : launch_pair<(GROUPED ? 256 : 192), GROUPED>(p, rows, W, stream);
 }
 
 template <int NR, bool FUSED>
 int launch_few(const FewProduct& p, const void* rows, const void* W, cudaStream_t stream) {
     using L = FewPlan<NR, FUSED>;
-    static bool configured = false;
-    if (!configured) {
-        const cudaError_t e = cudaFuncSetAttribute(mx4_few_kernel<NR, FUSED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   L::total(FEW_SLICE));
-        if (e != cudaSuccess) return (int)e;
-        configured = true;
-    }
+    static SharedLimit limit;
+    if (const int e = limit.set(mx4_few_kernel<NR, FUSED>, L::total(FEW_SLICE))) return e;
     CUtensorMap rows_map, w_map;
     if (!codes_map(W, p.N, p.K, UMMA_M, &w_map)) return MLS_ERR_TENSOR_MAP;
     if (FUSED) rows_map = w_map;                                 // (not read)
@@ -212,9 +202,9 @@ int launch_few(const FewProduct& p, const void* rows, const void* W, cudaStream_
 // One matrix.  rows_type >= 0: rows [M, K] of that type, ld values apart, that are quantised into a and sf_a first, or with
 // `fused` within the product; rows_type < 0: a and sf_a are there.  slice > 0: the product of few rows (M <= 16 with `fused`, else
 // 64), at most eight slices of so many times 256 of K.
-MLS_API int mls_mx4_product(int unit, const void* rows, int rows_type, long long ld, void* a, void* sf_a, const void* w,
-                            const void* sf_w, void* out, int out_type, int M, int N, int K, int slice, int fused, int early,
-                            float alpha, float limit, int* status, void* stream_) {
+static int product(int unit, const void* rows, int rows_type, long long ld, void* a, void* sf_a, const void* w, const void* sf_w,
+                   void* out, int out_type, int M, int N, int K, int slice, int fused, int early, float alpha, float limit,
+                   int* status, void* stream_) {
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0) return MLS_ERR_UNSUPPORTED;
     const cudaStream_t stream = (cudaStream_t)stream_;
@@ -246,11 +236,10 @@ MLS_API int mls_mx4_product(int unit, const void* rows, int rows_type, long long
 // Expert by expert: the slots of a routed step and w [E, 1 or 2, N, K].  The rows (sorted, or gathered from the tokens')
 // are quantised into a and sf_a first: `tokens` rows once each into t and sf_t and from there into their slots, or (tokens == 0)
 // every slot's by itself.
-MLS_API int mls_mx4_expert_product(int unit, const void* rows, int rows_type, long long ld, int top, int gather, int tokens,
-                                   void* t, void* sf_t, void* a, void* sf_a, const void* w, const void* sf_w, void* out,
-                                   int out_type, int n_slots, int n_experts, int N, int K, const int* order, const int* idx,
-                                   const int* offsets, const float* weight, int scale, float alpha, float limit, int* status,
-                                   void* stream_) {
+static int expert_product(int unit, const void* rows, int rows_type, long long ld, int top, int gather, int tokens, void* t,
+                          void* sf_t, void* a, void* sf_a, const void* w, const void* sf_w, void* out, int out_type,
+                          int n_slots, int n_experts, int N, int K, const int* order, const int* idx, const int* offsets,
+                          const float* weight, int scale, float alpha, float limit, int* status, void* stream_) {
     if (n_slots <= 0 || N <= 0 || n_experts <= 0) return 0;
     if (K <= 0 || top <= 0) return MLS_ERR_UNSUPPORTED;
     const cudaStream_t stream = (cudaStream_t)stream_;
@@ -275,4 +264,23 @@ MLS_API int mls_mx4_expert_product(int unit, const void* rows, int rows_type, lo
         if (rc) return rc;
     }
     return 0;
+}
+
+MLS_API int mls_mx4_product(int unit, const void* rows, int rows_type, long long ld, void* a, void* sf_a, const void* w,
+                            const void* sf_w, void* out, int out_type, int M, int N, int K, int slice, int fused, int early,
+                            float alpha, float limit, int* status, void* stream) {
+    return guarded([&] {
+        return product(unit, rows, rows_type, ld, a, sf_a, w, sf_w, out, out_type, M, N, K, slice, fused, early, alpha, limit,
+                       status, stream);
+    });
+}
+MLS_API int mls_mx4_expert_product(int unit, const void* rows, int rows_type, long long ld, int top, int gather, int tokens,
+                                   void* t, void* sf_t, void* a, void* sf_a, const void* w, const void* sf_w, void* out,
+                                   int out_type, int n_slots, int n_experts, int N, int K, const int* order, const int* idx,
+                                   const int* offsets, const float* weight, int scale, float alpha, float limit, int* status,
+                                   void* stream) {
+    return guarded([&] {
+        return expert_product(unit, rows, rows_type, ld, top, gather, tokens, t, sf_t, a, sf_a, w, sf_w, out, out_type, n_slots,
+                              n_experts, N, K, order, idx, offsets, weight, scale, alpha, limit, status, stream);
+    });
 }

@@ -41,7 +41,7 @@ class Engine:
         """An engine from an ``EngineOptions`` record (whose ``dtype``, ``kv_dtype`` and
         ``device`` must agree with how ``model`` was loaded)."""
         rt = model.runtime
-        options.check_against(str(rt.act_dtype).replace("torch.", ""), rt.device)
+        options.check_against(str(rt.act_dtype).replace("torch.", ""), rt.device, rt.ffn_weights)
         return cls(model, num_blocks=options.num_blocks, block_size=options.block_size,
                    max_batch=options.max_batch, max_tokens_per_step=options.max_tokens_per_step,
                    chunk_size=options.chunk_size, cuda_graphs=options.cuda_graphs,

@@ -24,28 +24,30 @@ class LLM:
 
     @classmethod
     def from_folder(cls, folder, dtype: str | None = None, device=None, options=None,
-                    **engine_options) -> "LLM":
+                    ffn_weights: str | None = None, **engine_options) -> "LLM":
         """``options`` (an ``EngineOptions``) also says in which dtype and on which device
-        the folder is loaded, unless ``dtype`` / ``device`` are given here."""
-        dtype, device = cls._where(dtype, device, options)
-        return cls(load_model(folder, dtype=dtype, device=device), options, **engine_options)
+        the folder is loaded and how its feed-forward weights are held, unless ``dtype`` / ``device`` /
+        ``ffn_weights`` are given here."""
+        dtype, device, ffn_weights = cls._where(dtype, device, ffn_weights, options)
+        return cls(load_model(folder, dtype=dtype, device=device, ffn_weights=ffn_weights), options, **engine_options)
 
     @classmethod
     def from_random(cls, config, seed: int = 0, norm_std: float = 0.0,
                     dtype: str | None = None, device=None, fast: bool = False, options=None,
-                    **engine_options) -> "LLM":
+                    ffn_weights: str | None = None, **engine_options) -> "LLM":
         if isinstance(config, dict):
             config = config_from_dict(config)
-        dtype, device = cls._where(dtype, device, options)
-        return cls(random_model(config, seed, norm_std, dtype, device, fast), options,
+        dtype, device, ffn_weights = cls._where(dtype, device, ffn_weights, options)
+        return cls(random_model(config, seed, norm_std, dtype, device, fast, ffn_weights), options,
                    **engine_options)
 
     @staticmethod
-    def _where(dtype, device, options):
+    def _where(dtype, device, ffn_weights, options):
         if options is not None:
             dtype = dtype or options.dtype
             device = device or options.device
-        return dtype, device or "cuda:0"
+            ffn_weights = ffn_weights or options.ffn_weights
+        return dtype, device or "cuda:0", ffn_weights
 
     def generate(self, prompts, max_new_tokens: int = 32, temperature: float = 0.0,
                  seed: int | None = None, eos=None) -> list:

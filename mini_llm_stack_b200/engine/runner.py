@@ -29,15 +29,16 @@ from .batch import BatchBuilder
 _TORCH_DTYPES = {"bfloat16": torch.bfloat16, "float32": torch.float32}
 
 
-def load_model(folder, dtype: str | None = None, device="cuda:0"):
-    """Model of a folder (config.json + model.safetensors), bound to a runtime."""
+def load_model(folder, dtype: str | None = None, device="cuda:0", ffn_weights: str | None = None):
+    """Model of a folder (config.json + model.safetensors), bound to a runtime; ``ffn_weights``: see
+    ``EngineOptions``."""
     config = config_from_folder(folder)
     if hasattr(config, "with_tensor_shapes"):
         # a design may leave sizes to its tensors' shapes: the file's header has them
         with open_weights(folder) as f:
             config = config.with_tensor_shapes({n: tuple(e.shape) for n, e in f.entries.items()})
     run_dtype = _TORCH_DTYPES[dtype or config.dtype]
-    runtime = Runtime(device, run_dtype)
+    runtime = Runtime(device, run_dtype, ffn_weights)
     model = build_model(config)
     tensors = load_tensors(folder, model.tensor_specs(), model.tied_names(), run_dtype,
                            runtime.device, aliases=model.name_aliases())
@@ -46,7 +47,7 @@ def load_model(folder, dtype: str | None = None, device="cuda:0"):
 
 
 def random_model(config, seed: int, norm_std: float = 0.0, dtype: str | None = None,
-                 device="cuda:0", fast: bool = False):
+                 device="cuda:0", fast: bool = False, ffn_weights: str | None = None):
     """Model with random weights, without a folder in between.
 
     The tensors are those ``write_random_model`` would store for the same
@@ -56,7 +57,7 @@ def random_model(config, seed: int, norm_std: float = 0.0, dtype: str | None = N
     """
     from ..weights.random_init import INIT_STD
     run_dtype = _TORCH_DTYPES[dtype or config.dtype]
-    runtime = Runtime(device, run_dtype)
+    runtime = Runtime(device, run_dtype, ffn_weights)
     model = build_model(config)
     tensors = {}
     if fast:

@@ -15,6 +15,7 @@ import os
 
 import torch
 
+from ..config.engine_options import check_ffn_weights
 from . import library
 
 _P = ctypes.c_void_p
@@ -25,6 +26,9 @@ _LL = ctypes.c_longlong
 _ERRORS = {100001: "a size this kernel does not support",
            100002: "the driver refused to encode a tensor map"}
 
+
+# (the same for the current device's number)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
 # torch's own fast path to the current stream's handle (a C call without the argument
 # handling of torch.cuda.current_stream, which costs several microseconds a launch)
@@ -162,7 +166,7 @@ class Mx4:
         0: the tiles alone are more, the product takes the way of many rows.  (In us, this way and that one: 8 rows, 4,096
         outputs of 14,336 in eight slices 9.3 and 20.8, 28,672 of 4,096 in one 14.4 and 17.5.  From 17 rows on one or two slices
         do not pay: 32 rows, 28,672 of 4,096 16.9 and 16.3, 7,168 of 4,096 in four slices 8.4 and 9.3.)"""
-        steps, tiles = -(-k // 256), -(-n // 128)
+        steps, tiles = -(-k // 256), max(1, -(-n // 128))
         slices = min(8, steps, 2 * sm_count * 19 // 20 // tiles)
         return -(-steps // slices) if slices else 0
 
@@ -1463,7 +1467,8 @@ class Ops:
             shared.release()
 
     # ------------------------------------------------- 4-bit microscaled rows and weights
-    MX4_MOST_K = 1 << 20
+    MX4_MOST_K = 1 << 20     # values of a row
+    MX4_MOST_ROWS = 1 << 28  # rows of a matrix, and of a weight's matrices together
     MX4_ONCE = 1 << 16       # slots x steps of 256 of K from which on tokens are quantised once
     MX4_FUSED_TASKS = 64     # 256 values of a row each: with so many a block the product quantises its rows itself
 
@@ -1471,8 +1476,15 @@ class Ops:
         for t in tensors:
             if t.get_device() != self._device_index:
                 raise KernelError(f"{what}: tensors must be on {self.device}")
-        if torch.cuda.current_device() != self._device_index:
+        if _current_device() != self._device_index:
             raise KernelError(f"{what}: {self.device} must be the current device")
+
+    @staticmethod
+    def _mx4_apart(rows, ld: int, out, what: str) -> None:
+        """A product's blocks read rows while others store outputs already."""
+        a, b, (m, k) = rows.data_ptr(), out.data_ptr(), rows.shape
+        if a < b + out.numel() * out.element_size() and b < a + ((m - 1) * ld + k) * rows.element_size():
+            raise KernelError(f"{what}: the output lies where the rows are")
 
     @staticmethod
     def _mx4_type(t, what: str) -> int:
@@ -1501,8 +1513,9 @@ class Ops:
         what = "quantize_mx4"
         shape = tuple(x.shape)
         code = self._mx4_type(x, what)
-        if len(shape) < 2 or not 1 <= shape[-1] <= self.MX4_MOST_K:
-            raise KernelError(f"{what}: matrices [..., rows, K] with K from 1 to {self.MX4_MOST_K}, not {shape}")
+        if len(shape) < 2 or not 1 <= shape[-1] <= self.MX4_MOST_K or x.numel() // shape[-1] > self.MX4_MOST_ROWS:
+            raise KernelError(f"{what}: matrices [..., rows, K] with K from 1 to {self.MX4_MOST_K} and at most "
+                              f"{self.MX4_MOST_ROWS} rows, not {shape}")
         if gate_up and (len(shape) < 3 or shape[-3] != 2):
             raise KernelError(f"{what}: gate_up goes with matrices [..., 2, N, K], not {shape}")
         self._mx4_here(what, x)
@@ -1573,9 +1586,11 @@ class Ops:
             raise KernelError(f"{what}: the weight comes from prepare_weight_mx4, "
                               + ("[2, N, K] with gate_up" if unit == 1 else "[N, K]"))
         shape, n, k = a.shape, w.n, w.k
-        m = shape[0]
-        if len(shape) != 2 or shape[1] != k or out.shape != (m, n) or not out.is_contiguous():
+        if len(shape) != 2 or shape[1] != k or out.shape != (shape[0], n) or not out.is_contiguous():
             raise KernelError(f"{what}: shapes do not fit")
+        m = shape[0]
+        if m > self.MX4_MOST_ROWS:
+            raise KernelError(f"{what}: at most {self.MX4_MOST_ROWS} rows")
         out_type = self._mx4_type(out, what)
         ready = a.__class__ is Mx4
         self._mx4_here(what, a.data if ready else a, w.data, out)
@@ -1592,6 +1607,7 @@ class Ops:
             codes, scales = a.codes_at, a.scales_at
         else:
             code, ld, rows = self._mx4_type(a, what), self._mx4_ld(a, k, what), a.data_ptr()
+            self._mx4_apart(a, ld, out, what)
             fused = 0 < few <= 12 and m <= 16 and m * few <= self.MX4_FUSED_TASKS
             if not fused:
                 codes, scales, _, _ = self._mx4_scratch(m, k, (m + 127) // 128)
@@ -1640,6 +1656,9 @@ class Ops:
         self._mx4_here(what, rows, w.data, out, order, idx, offsets, weight)
         if slots == 0 or n_experts == 0 or n == 0:
             return
+        if slots > self.MX4_MOST_ROWS:
+            raise KernelError(f"{what}: at most {self.MX4_MOST_ROWS} slots")
+        self._mx4_apart(rows, ld, out, what)
         # (many slots: every token is quantised once and copied to its slots; 12,288 slots of 2,048 tokens x 4,096 in 12 us
         # where they took 27 one by one)
         tokens = shape[0] if unit and top > 1 and slots * -(-k // 256) >= self.MX4_ONCE else 0
@@ -2315,9 +2334,10 @@ class Runtime:
     residual_dtype = torch.float32
     logits_dtype = torch.float32
 
-    def __init__(self, device="cuda:0", dtype: torch.dtype = torch.bfloat16):
+    def __init__(self, device="cuda:0", dtype: torch.dtype = torch.bfloat16, ffn_weights: str | None = None):
         self.device = torch.device(device)
         self.act_dtype = dtype
+        self.ffn_weights = check_ffn_weights(ffn_weights)      # how feed-forwards hold their weights (None: as loaded)
         self.ops = Ops(self.device, dtype)
         self._buffers: dict = {}
         self._views: dict = {}               # (tag, dtype, shape) -> the view handed out last time

@@ -14,6 +14,22 @@ import torch
 from .base import FeedForward, StepContext, TensorSpec
 
 
+def _four_bit(runtime) -> bool:
+    """Whether the runtime's feed-forwards hold their weights, and multiply their rows, as 4-bit microscaled values
+    (``EngineOptions.ffn_weights``); builds the kernels if so."""
+    if getattr(runtime, "ffn_weights", None) != "mxfp4":
+        return False
+    runtime.ops.require_part("mx4")
+    return True
+
+
+def _pair(gate, up):
+    """A gate and an up matrix (or the experts' ``[E, N, K]``) as one tensor ``[..., 2, N, K]``."""
+    if gate.dtype != up.dtype:
+        gate, up = gate.float(), up.float()
+    return torch.stack([gate, up], dim=-3)
+
+
 class SwiGLUFeedForward(FeedForward):
     decode_capturable = prompt_capturable = True   # forward only launches kernels on the current stream
 
@@ -36,6 +52,11 @@ class SwiGLUFeedForward(FeedForward):
         if parts[0].dtype != parts[1].dtype:
             parts = [p.float() for p in parts]
         ops = runtime.ops
+        self.four_bit = _four_bit(runtime)
+        if self.four_bit:
+            self.w_gate_up = ops.prepare_weight_mx4(_pair(*parts), gate_up=True)
+            self.w_down = ops.prepare_weight_mx4(tensors["w_down.weight"])
+            return
         # one kernel for projection and activation where the tensor-core kernel takes
         # the sizes: its weight holds gate and up rows interleaved in blocks of 16
         self.fused = (parts[0].dtype == torch.bfloat16
@@ -51,6 +72,11 @@ class SwiGLUFeedForward(FeedForward):
         t = h.shape[0]
         i = self.intermediate_size
         act = rt.buffer("ffn_act", (t, i), rt.act_dtype)
+        if self.four_bit:
+            delta = rt.buffer("delta", (t, self.d_model), rt.act_dtype)
+            rt.ops.linear_glu_mx4(h, self.w_gate_up, act)
+            rt.ops.linear_mx4(act, self.w_down, delta)
+            return delta
         if self.fused:
             rt.ops.linear_swiglu(h, self.w_gate_up, act)
         else:
@@ -84,6 +110,13 @@ class ClampedGLUFeedForward(FeedForward):
         self.runtime = runtime
         g, u, dn = self.names
         ops = runtime.ops
+        self.four_bit = _four_bit(runtime)
+        if self.four_bit:
+            if not self.limit > 0:
+                raise ValueError("a clamped unit in 4 bits needs a limit")
+            self.w_gate_up = ops.prepare_weight_mx4(_pair(tensors[g], tensors[u]), gate_up=True)
+            self.w_down = ops.prepare_weight_mx4(tensors[dn])
+            return
         self.fused = (tensors[g].dtype == torch.bfloat16 and tensors[u].dtype == torch.bfloat16
                       and ops.can_fuse_swiglu(self.d_model, self.intermediate_size))
         if self.fused:
@@ -96,6 +129,11 @@ class ClampedGLUFeedForward(FeedForward):
         rt = self.runtime
         t, i = h.shape[0], self.intermediate_size
         act = rt.buffer("ffn_act", (t, i), rt.act_dtype)
+        if self.four_bit:
+            delta = rt.buffer("delta", (t, self.d_model), rt.act_dtype)
+            rt.ops.linear_glu_mx4(h, self.w_gate_up, act, alpha=self.alpha, limit=self.limit)
+            rt.ops.linear_mx4(act, self.w_down, delta)
+            return delta
         if self.fused:
             rt.ops.linear_clamped_glu(h, self.w_gate_up, act, self.alpha, self.limit)
         else:
@@ -134,29 +172,37 @@ class SquaredReluFeedForward(FeedForward):
 
     def bind(self, tensors: dict, runtime) -> None:
         self.runtime = runtime
-        self.w_up = runtime.ops.prepare_weight(tensors[self.names[0]])
-        self.w_down = runtime.ops.prepare_weight(tensors[self.names[1]])
+        self.four_bit = _four_bit(runtime)
+        prepare = runtime.ops.prepare_weight_mx4 if self.four_bit else runtime.ops.prepare_weight
+        self.w_up = prepare(tensors[self.names[0]])
+        self.w_down = prepare(tensors[self.names[1]])
         if self.biases:
             self.b_up = tensors[f"{self.names[0]}.b"].contiguous()
             self.b_down = tensors[f"{self.names[1]}.b"].contiguous()
-        self.fused = (self.w_up.dtype == torch.bfloat16
+        self.fused = (not self.four_bit and self.w_up.dtype == torch.bfloat16
                       and runtime.ops.can_fuse_activation(self.d_model))
 
     def forward(self, h, step: StepContext):
         rt = self.runtime
         t = h.shape[0]
         act = rt.buffer("ffn_act", (t, self.intermediate_size), rt.act_dtype)
+        linear = rt.ops.linear_mx4 if self.four_bit else rt.ops.linear
         if self.fused:
             rt.ops.linear_relu_squared(h, self.w_up, act, bias=self.b_up)
         elif self.b_up is not None:
             z = rt.buffer("ffn_up", (t, self.intermediate_size), torch.float32)
-            rt.ops.linear(h, self.w_up, z)
+            linear(h, self.w_up, z)
             rt.ops.relu_squared(z, act, bias=self.b_up)
+        elif self.four_bit:
+            rt.ops.linear_relu_squared_mx4(h, self.w_up, act)
         else:
             rt.ops.linear(h, self.w_up, act)
             rt.ops.relu_squared(act, act)
         delta = rt.buffer("delta", (t, self.d_model), rt.act_dtype)
-        delta = rt.ops.linear_parts(act, self.w_down, delta)
+        if self.four_bit:
+            linear(act, self.w_down, delta)
+        else:
+            delta = rt.ops.linear_parts(act, self.w_down, delta)
         return (delta, self.b_down) if self.b_down is not None else delta
 
 
@@ -251,12 +297,22 @@ class RoutedExperts(FeedForward):
             self.correction = tensors["correction"].float().contiguous()
         if self.router_bias:
             self.correction = tensors["router.b"].float().contiguous()
-        if self.unit == "gated":
+        self.four_bit = _four_bit(runtime)
+        if self.four_bit:
+            def stack(name):
+                return torch.stack([tensors[f"e{i}.{name}"] for i in range(n)])
+            if self.unit == "gated":
+                self.w_gate_up = runtime.ops.prepare_weight_mx4(_pair(stack("gate"), stack("up")), gate_up=True)
+            else:
+                self.w_up = runtime.ops.prepare_weight_mx4(stack("up"))
+            self.w_down = runtime.ops.prepare_weight_mx4(stack("down"))
+        elif self.unit == "gated":
             self.w_gate_up = torch.stack([torch.cat([tensors[f"e{i}.gate"], tensors[f"e{i}.up"]], 0)
                                           for i in range(n)]).contiguous()
         else:
             self.w_up = torch.stack([tensors[f"e{i}.up"] for i in range(n)]).contiguous()
-        self.w_down = torch.stack([tensors[f"e{i}.down"] for i in range(n)]).contiguous()
+        if not self.four_bit:
+            self.w_down = torch.stack([tensors[f"e{i}.down"] for i in range(n)]).contiguous()
         if self.shared is not None:
             self.shared.bind({k[len("shared."):]: v for k, v in tensors.items()
                               if k.startswith("shared.") and k != "shared.sg"}, runtime)
@@ -287,12 +343,13 @@ class RoutedExperts(FeedForward):
         n_slots = t * self.top
         y = rt.buffer("expert_act", (n_slots, self.expert_size), rt.act_dtype)
         per_slot = rt.buffer("expert_out", (n_slots, self.d_model), torch.float32)
+        glu, relu_squared, down = ((ops.expert_glu_mx4, ops.expert_relu_squared_mx4, ops.expert_down_mx4) if self.four_bit
+                                   else (ops.expert_glu, ops.expert_relu_squared, ops.expert_down))
         if self.unit == "gated":
-            ops.expert_glu(h, self.w_gate_up, y, work, self.top, self.weigh == "input",
-                           alpha=self.alpha, limit=self.limit)
+            glu(h, self.w_gate_up, y, work, self.top, self.weigh == "input", alpha=self.alpha, limit=self.limit)
         else:
-            ops.expert_relu_squared(h, self.w_up, y, work, self.top, self.weigh == "input")
-        ops.expert_down(y, self.w_down, per_slot, work, self.top, self.weigh == "output")
+            relu_squared(h, self.w_up, y, work, self.top, self.weigh == "input")
+        down(y, self.w_down, per_slot, work, self.top, self.weigh == "output")
         shared = None
         if self.shared is not None:
             shared = self.shared.forward(h, step)    # (maybe left as its product's K-parts)

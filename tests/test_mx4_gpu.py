@@ -226,3 +226,226 @@ def test_products_by_expert(ops, t, experts, identity, top, d, f, spread, kind):
         z, off = plain.product(qy[at], plain.nearest(w2[e]))
         s = torch.ones((), dtype=torch.float64) if scale_in else share[slot, None]
         near(out[slot], z * s, (off + z.abs() * plain.STEPS) * s, torch.float32)
+
+
+# ------------------------------------------------------------------------------------- more than one round of tiles
+def on_device(x):
+    """nearest() on the device: scales by frexp, which is exact."""
+    k = x.shape[-1]
+    v = torch.nn.functional.pad(x.double(), (0, -k % 32)).unflatten(-1, (-1, 32))
+    top = v.abs().amax(-1, keepdim=True)
+    scale = torch.ldexp(torch.ones_like(top), (torch.frexp(top).exponent - 3).clamp(min=-127))
+    v = v / torch.where(top > 0, scale, 1.0)
+    step = torch.where(v.abs() < 2, 0.5, torch.where(v.abs() < 4, 1.0, 2.0).double())
+    return ((torch.round(v / step) * step).clamp(-6, 6) * torch.where(top > 0, scale, 1.0)).flatten(-2)[..., :k]
+
+
+@pytest.mark.parametrize("m, n, k", [(65, 40000, 300), (150, 20500, 520), (260, 19000, 1100), (300, 15000, 300), (700, 9100, 700),
+                                     (1500, 3000, 3300), (2050, 4100, 2600), (513, 700, 9000), (20000, 130, 300)])
+@pytest.mark.parametrize("gated", [False, True])
+def test_many_tiles(ops, m, n, k, gated):
+    g = torch.Generator("cuda").manual_seed(m + n + k)
+    a = torch.randn(m, k, generator=g, device="cuda").bfloat16()
+    w = (torch.randn(2 if gated else 1, n, k, generator=g, device="cuda") * k ** -0.5).bfloat16()
+    out = torch.full((m, n), float("nan"), dtype=torch.bfloat16, device="cuda")
+    if gated:
+        ops.linear_glu_mx4(a, ops.prepare_weight_mx4(w, gate_up=True), out)
+    else:
+        ops.linear_mx4(a, ops.prepare_weight_mx4(w[0]), out)
+    ops.check_status()
+    qa, qw = on_device(a), on_device(w)
+    z, off = plain.product(qa, qw[0])
+    if gated:
+        z, off = plain.unit(z, plain.product(qa, qw[1])[0], off, plain.product(qa, qw[1])[1])
+    far = (out.double() - z).abs() - off - plain.rounding(torch.bfloat16, z)
+    assert bool((far <= 0).all()), float(far.max())
+
+
+@pytest.mark.parametrize("t, experts, top, d, f", [(1200, 12, 4, 1100, 1000), (900, 3, 2, 700, 3000), (64, 60, 6, 1030, 600)])
+def test_many_tiles_by_expert(ops, t, experts, top, d, f):
+    g = torch.Generator("cuda").manual_seed(t)
+    h = torch.randn(t, d, generator=g, device="cuda").bfloat16()
+    w1 = (torch.randn(experts, 2, f, d, generator=g, device="cuda") * d ** -0.5).bfloat16()
+    w2 = (torch.randn(experts, d, f, generator=g, device="cuda") * f ** -0.5).bfloat16()
+    liked = torch.randn(t, experts, generator=g, device="cuda") + 2 * torch.randn(experts, generator=g, device="cuda")
+    idx = liked.topk(top).indices
+    work = routed(idx.cpu(), torch.softmax(torch.randn(t, top, generator=g, device="cuda"), 1).cpu(), experts)
+    y = torch.full((t * top, f), float("nan"), dtype=torch.bfloat16, device="cuda")
+    out = torch.full((t * top, d), float("nan"), device="cuda")
+    ops.expert_glu_mx4(h, ops.prepare_weight_mx4(w1, gate_up=True), y, work, top, False)
+    ops.expert_down_mx4(y, ops.prepare_weight_mx4(w2), out, work, top, True)
+    ops.check_status()
+    order, share = work["order"].long(), work["weight"].double()
+    qh, qy, flat = on_device(h), on_device(y), idx.reshape(-1)
+    for e in range(experts):
+        at = (flat[order] == e).nonzero()[:, 0]
+        if at.numel() == 0:
+            continue
+        slot, qw = order[at], on_device(w1[e])
+        gate, up = (plain.product(qh[slot // top], m) for m in qw)
+        want, off = plain.unit(gate[0], up[0], gate[1], up[1])
+        assert bool(((y[at].double() - want).abs() <= off + plain.rounding(torch.bfloat16, want)).all()), e
+        want, off = plain.product(qy[at], on_device(w2[e]))
+        s = share[slot, None]
+        far = (out[slot].double() - want * s).abs() - (off + want.abs() * plain.STEPS) * s - plain.rounding(torch.float32, want * s)
+        assert bool((far <= 0).all()), (e, float(far.max()))
+
+
+# ------------------------------------------------------------------------------------- what is no number
+@pytest.mark.parametrize("m, n, k", [(3, 200, 300), (20, 200, 300), (40, 200, 2300), (100, 300, 300), (300, 300, 600),
+                                     (600, 2100, 300)])
+def test_what_is_no_number_stays_in_its_row(ops, m, n, k):
+    a, w = dense_inputs(m, n, k, 1)
+    want, off = plain.product(plain.nearest(a), plain.nearest(w[0]))
+    bad_rows = {0: float("nan"), m // 2: float("inf"), m - 1: float("-inf")}
+    for r, v in bad_rows.items():
+        a[r, (7 * r) % k] = v
+    w[0, n // 3, k - 1] = float("inf")
+    out = torch.empty((m, n), dtype=torch.bfloat16, device="cuda")
+    ops.linear_mx4(a.cuda(), ops.prepare_weight_mx4(w[0].cuda()), out)
+    ops.check_status()
+    out = out.cpu()
+    bad = torch.zeros(m, n, dtype=torch.bool)
+    bad[list(bad_rows)] = True
+    bad[:, n // 3] = True
+    assert bool(out[bad].isnan().all())
+    assert bool(((out.double() - want).abs() <= off + plain.rounding(torch.bfloat16, want))[~bad].all())
+
+
+def test_what_is_no_number_stays_with_its_slots(ops):
+    t, experts, top, d, f = 70, 4, 2, 96, 64
+    g = gen("nan experts")
+    idx = choices(t, experts, top, "one", g)
+    work = routed(idx, torch.ones(t, top), experts)
+    h = torch.randn(t, d, generator=g).bfloat16()
+    h[5, 90] = float("nan")
+    w = (torch.randn(experts, 2, f, d, generator=g) * d ** -0.5).bfloat16()
+    w[2, 0, 0, 0] = float("nan")
+    y = torch.zeros((t * top, f), dtype=torch.bfloat16, device="cuda")
+    ops.expert_glu_mx4(h.cuda(), ops.prepare_weight_mx4(w.cuda(), gate_up=True), y, work, top, False)
+    order = work["order"].cpu().long()
+    bad = torch.zeros(t * top, f, dtype=torch.bool)
+    bad[order // top == 5] = True
+    bad[idx.reshape(-1)[order] == 2, 0] = True
+    assert torch.equal(y.isnan().cpu(), bad)
+
+
+# ------------------------------------------------------------------------------------- how calls may be made
+def test_empty_calls_and_edges(ops):
+    w = ops.prepare_weight_mx4(torch.randn(40, 64, device="cuda"))
+    ops.linear_mx4(torch.empty(0, 64, device="cuda"), w, torch.empty(0, 40, device="cuda"))
+    q = ops.quantize_mx4(torch.empty(0, 64, device="cuda"))
+    assert q.shape == (0, 64) and q.codes.shape == (0, 32)
+    ops.mx4_values(q, torch.empty(0, 64, device="cuda"))
+    pairs = ops.prepare_weight_mx4(torch.randn(2, 2, 24, 64, device="cuda"), gate_up=True)
+    work = routed(torch.empty(0, 1, dtype=torch.long), torch.empty(0, 1), 2)
+    ops.expert_glu_mx4(torch.empty(0, 64, device="cuda"), pairs, torch.empty(0, 24, device="cuda"), work, 1, False)
+    ops.check_status()
+
+
+@pytest.mark.parametrize("m", [1, 12, 40, 150, 400])
+def test_nothing_beside_the_output_is_written(ops, m):
+    n, k = 330, 700
+    a, w = dense_inputs(m, n, k, 2)
+    room = torch.full((m + 4, n), 9.0, dtype=torch.bfloat16, device="cuda")
+    ops.linear_mx4(a.cuda(), ops.prepare_weight_mx4(w[0].cuda()), room[2:-2])
+    ops.linear_glu_mx4(a.cuda(), ops.prepare_weight_mx4(w.cuda(), gate_up=True), room[2:-2])
+    ops.check_status()
+    assert bool((room[:2] == 9).all()) and bool((room[-2:] == 9).all()) and not bool((room[2:-2] == 9).all())
+
+
+@pytest.mark.parametrize("m", [1, 8, 12, 40, 100, 300, 900])
+def test_the_same_bits_each_time_and_on_another_stream(ops, m):
+    a, w = dense_inputs(m, 1000, 2100, 1)
+    a, held = a.cuda(), ops.prepare_weight_mx4(w[0].cuda())
+    outs = []
+    side = torch.cuda.Stream()
+    for stream in (torch.cuda.current_stream(), torch.cuda.current_stream(), side):
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            out = torch.full((m, 1000), float("nan"), device="cuda")
+            ops.linear_mx4(a, held, out)
+        torch.cuda.current_stream().wait_stream(stream)
+        outs.append(out)
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_rows_with_a_stride(ops):
+    for m in (5, 30, 200):
+        big = torch.randn(m, 900, generator=gen("stride", m)).bfloat16().cuda()
+        w = ops.prepare_weight_mx4(torch.randn(72, 300, generator=gen("w")).bfloat16().cuda())
+        for view in (big[:, 8:308], big[:, 301:601], big[:, ::1][:, 600:]):
+            out, want = torch.empty(m, 72, device="cuda"), torch.empty(m, 72, device="cuda")
+            ops.linear_mx4(view, w, out)
+            ops.linear_mx4(view.contiguous(), w, want)
+            assert torch.equal(out, want)
+
+
+def test_graphs_keep_their_memory(ops):
+    """Captured calls, replayed behind calls that need more scratch memory, and on other inputs."""
+    own = Runtime("cuda:0", torch.bfloat16).ops
+    g = gen("graph")
+    cases = []
+    for m, n, k in ((6, 300, 600), (50, 300, 600), (400, 300, 600)):
+        a = torch.randn(m, k, generator=g).bfloat16().cuda()
+        w = own.prepare_weight_mx4(torch.randn(n, k, generator=g).bfloat16().cuda())
+        cases.append((a, w, torch.empty(m, n, device="cuda")))
+    t, experts, top = 90, 5, 2
+    idx = choices(t, experts, top, "even", g)
+    work = routed(idx, torch.ones(t, top), experts)
+    h = torch.randn(t, 200, generator=g).bfloat16().cuda()
+    w1 = own.prepare_weight_mx4(torch.randn(experts, 2, 64, 200, generator=g).bfloat16().cuda(), gate_up=True)
+    y = torch.empty(t * top, 64, dtype=torch.bfloat16, device="cuda")
+
+    def run():
+        for a, w, out in cases:
+            own.linear_mx4(a, w, out)
+        own.expert_glu_mx4(h, w1, y, work, top, False)
+
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    big = torch.randn(3000, 4096, device="cuda").bfloat16()
+    wide = own.prepare_weight_mx4(torch.randn(64, 4096, device="cuda"))
+    own.linear_mx4(big, wide, torch.empty(3000, 64, device="cuda"))      # the scratch memory moves
+    for a, _, _ in cases:
+        a.copy_(torch.randn(a.shape, generator=g).bfloat16())
+    h.copy_(torch.randn(h.shape, generator=g).bfloat16())
+    filled = [torch.full((1 << 20,), 0xff, dtype=torch.uint8, device="cuda") for _ in range(64)]
+    graph.replay()
+    got = [out.clone() for _, _, out in cases] + [y.clone()]
+    run()
+    torch.cuda.synchronize()
+    for a, b in zip(got, [out for _, _, out in cases] + [y]):
+        assert torch.equal(a, b)
+    assert all(bool((f == 0xff).all()) for f in filled)
+
+
+def test_weights_written_anew_are_waited_for(ops):
+    """A product right behind the quantisation of its weights, where kernels start under their predecessors."""
+    g = gen("anew")
+    a = torch.randn(4, 2048, generator=g).bfloat16().cuda()
+    first, second = (torch.randn(4096, 2048, generator=g).bfloat16().cuda() for _ in range(2))
+    out, want = torch.empty(4, 4096, device="cuda"), torch.empty(4, 4096, device="cuda")
+    ops.linear_mx4(a, ops.prepare_weight_mx4(second), want)
+    held = ops.prepare_weight_mx4(first)
+    for _ in range(20):
+        ops.quantize_mx4(first, into=held)
+        ops.quantize_mx4(second, into=held)
+        ops.linear_mx4(a, held, out)
+    assert torch.equal(out, want)
+
+
+def test_refusals(ops):
+    w = ops.prepare_weight_mx4(torch.randn(40, 64, device="cuda"))
+    a, out = torch.randn(3, 64, device="cuda"), torch.empty(3, 40, device="cuda")
+    both = torch.zeros(400, device="cuda")
+    for call in (lambda: ops.linear_mx4(a.cpu(), w, out), lambda: ops.linear_mx4(a, w, out.cpu()),
+                 lambda: ops.linear_mx4(both[:192].view(3, 64), w, both[100:220].view(3, 40)),
+                 lambda: ops.quantize_mx4(a.cpu()), lambda: ops.mx4_values(w, torch.empty(40, 64)),
+                 lambda: ops.linear_mx4(ops.quantize_mx4(torch.randn(2, 3, 64, device="cuda")), w, out)):
+        with pytest.raises(KernelError):
+            call()
+    ops.linear_mx4(a, w, out)
+    ops.check_status()

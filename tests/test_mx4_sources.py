@@ -1,0 +1,53 @@
+"""The rules of test_kernel_sources.py for the kernels on 4-bit values, whose bodies are functions of headers."""
+
+import re
+
+import pytest
+
+from test_kernel_sources import CSRC, roles
+
+HEADERS = {"mx4_gemm.h": "product_block", "mx4_few.h": "few_block", "mx4_pair.h": "pair_block"}
+
+
+def block(header):
+    text = re.sub(r"//[^\n]*", "", (CSRC / header).read_text())
+    body = text[text.index(f"void {HEADERS[header]}("):]
+    return body[:body.index("\n}\n")]
+
+
+def test_every_kernel_with_tensor_memory_is_known():
+    found = {p.name for p in CSRC.glob("mx4*") if "tmem_alloc" in p.read_text()}
+    assert found == set(HEADERS)
+
+
+@pytest.mark.parametrize("header", sorted(HEADERS))
+def test_successors_start_behind_the_allocation(header):
+    body = block(header)
+    assert body.count("chain_release();") == 1
+    assert re.search(r"if \(warp == \d\) \{\s*tmem_alloc(_pair)?\([^;]*;\s*chain_release\(\);\s*\}", body)
+    assert body.count("tmem_dealloc") == 1
+
+
+@pytest.mark.parametrize("header", sorted(HEADERS))
+def test_lanes_leave_a_loop_together(header):
+    for role in roles(block(header)):
+        if not re.search(r"mbar_wait\w*\(", role):
+            continue
+        together = re.search(r"elect_one|tmem_ld|store_unit|store_rows|_sync\(0xffffffffu|__syncwarp", role)
+        if together and "lane == 0) {\n" not in role[:250]:
+            assert not re.search(r"mbar_wait(_cluster)?\(", role), "a wait that each lane judges by itself"
+
+
+@pytest.mark.parametrize("header", sorted(HEADERS))
+def test_copies_land_before_the_block_ends(header):
+    parts = re.split(r"\n    (?:if|\} else if) \(warp ", block(header))
+    role = next(r for r in parts if re.search(r"tma_load_[23]d", r))
+    behind = role[max(m.end() for m in re.finditer(r"(tma_load_[23]d\w*|load_weights|load_rows)\(", role)):]
+    assert re.search(r"for \(int \w+ = [^;]*;[^)]*\)\s*if \(!mbar_wait\w*\([^;]*full[^;]*timed_out = true;", behind)
+
+
+def test_every_wait_is_bounded():
+    for p in CSRC.glob("mx4*"):
+        text = re.sub(r"//[^\n]*", "", p.read_text())
+        assert not re.search(r"while \(!?\s*mbar_|for \(;;\)|__nanosleep", text), p.name
+        assert "multicast::cluster" not in text, p.name
