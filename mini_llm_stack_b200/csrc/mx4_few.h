@@ -13,6 +13,7 @@ namespace mls_mx4 {
 constexpr int FEW_STAGES = 4;
 constexpr int FEW_WORKERS = 8;                        // warps that quantise, read the sums and store them
 constexpr int FEW_THREADS = 32 * (2 + FEW_WORKERS);
+constexpr int FEW_SLICES = 8;                         // blocks of a cluster, at most
 constexpr int FEW_SLICE = 12;                         // stages of K of a slice, at most (FUSED: two blocks an SM)
 
 struct FewProduct {
@@ -51,7 +52,7 @@ struct FewPlan {
 __device__ __forceinline__ float load_cluster_f32(uint32_t addr, uint32_t cta) {
     float v;
     asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}"
-                 : "=f"(v) : "r"(addr), "r"(cta) : "memory");
+                 : "=f"(v) : "r"(addr), "r"(cta));
     return v;
 }
 
@@ -231,10 +232,17 @@ __device__ __forceinline__ void few_block(const FewProduct& p, const CUtensorMap
             const int n = (pairs ? n0 / 2 : n0) + j;
             if (n >= p.width) continue;
             const uint32_t at = sums + 4 * (r * UMMA_M + (pairs ? (j / 16) * 32 + j % 16 : j));
-            float v = 0.f, u = 0.f;
-            for (int s = 0; s < slices; ++s) {
-                v += load_cluster_f32(at, s);
-                if (pairs) u += load_cluster_f32(at + 64, s);
+            // (all slices' sums are on their way before the first is added)
+            float v = 0.f, u = 0.f, vs[FEW_SLICES], us[FEW_SLICES];
+#pragma unroll
+            for (int s = 0; s < FEW_SLICES; ++s) {
+                if (s < slices) vs[s] = load_cluster_f32(at, s);
+                if (s < slices && pairs) us[s] = load_cluster_f32(at + 64, s);
+            }
+#pragma unroll
+            for (int s = 0; s < FEW_SLICES; ++s) {
+                if (s < slices) v += vs[s];
+                if (s < slices && pairs) u += us[s];
             }
             if (pairs) v = p.out_type == MLS_BF16 ? unit_of_sums<__nv_bfloat16>(v, u, p.alpha, p.limit)
                                                   : unit_of_sums<float>(v, u, p.alpha, p.limit);

@@ -33,10 +33,10 @@ mx4_product_kernel(const Product p, const __grid_constant__ CUtensorMap rows_map
 }
 
 template <int NT, bool GROUPED>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__((PairPlan<NT, GROUPED>::THREADS), 1)
-mx4_pair_kernel(const Product p, const __grid_constant__ CUtensorMap m_map, const __grid_constant__ CUtensorMap n_map,
-                const __grid_constant__ CUtensorMap sf_m_map, const __grid_constant__ CUtensorMap sf_n_map) {
-    pair_block<NT, GROUPED>(p, &m_map, &n_map, &sf_m_map, &sf_n_map);
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairPlan<NT>::THREADS, 1)
+mx4_pair_kernel(const Product p, const __grid_constant__ CUtensorMap rows_map, const __grid_constant__ CUtensorMap w_map,
+                const __grid_constant__ CUtensorMap sf_rows_map, const __grid_constant__ CUtensorMap sf_w_map) {
+    pair_block<NT, GROUPED>(p, &rows_map, &w_map, &sf_rows_map, &sf_w_map);
 }
 
 template <int NR, bool FUSED>
@@ -120,33 +120,27 @@ int launch_nt(const Product& p, const void* rows, const void* W, cudaStream_t st
 
 template <int NT, bool GROUPED>
 int launch_pair(const Product& p, const void* rows, const void* W, cudaStream_t stream) {
-    using L = PairPlan<NT, GROUPED>;
+    using L = PairPlan<NT>;
     static SharedLimit limit;
     if (const int e = limit.set(mx4_pair_kernel<NT, GROUPED>, L::FIXED + 4 * (TABLE_EXPERTS + 1))) return e;
     const long long row_tiles = GROUPED ? p.M / TILE_ROWS + p.all_experts + 1 : (p.M + TILE_ROWS - 1) / TILE_ROWS;
     const long long w_tiles = (long long)p.n_experts * ((p.N + TILE_ROWS - 1) / TILE_ROWS);
     CUtensorMap rows_map, w_map, sf_rows_map, sf_w_map;
-    if (!codes_map(rows, p.M, p.K, GROUPED ? L::BOX : UMMA_M, &rows_map) ||
-        !codes_map(W, (long long)p.n_experts * p.N, p.K, GROUPED ? UMMA_M : L::BOX, &w_map) ||
-        !scales_map(p.sf_a, row_tiles, p.K, GROUPED ? 2 : 1, &sf_rows_map) ||
-        !scales_map(p.sf_w, w_tiles, p.K, GROUPED ? 1 : 2, &sf_w_map))
+    if (!codes_map(rows, p.M, p.K, UMMA_M, &rows_map) || !codes_map(W, (long long)p.n_experts * p.N, p.K, NT / 2, &w_map) ||
+        !scales_map(p.sf_a, row_tiles, p.K, 1, &sf_rows_map) || !scales_map(p.sf_w, w_tiles, p.K, 2, &sf_w_map))
         return MLS_ERR_TENSOR_MAP;
-    constexpr int ROW_TILE = GROUPED ? NT : L::MT, W_TILE = GROUPED ? L::MT : NT;
-    const long long tiles = GROUPED ? (long long)(p.M / ROW_TILE) + (p.M < p.n_experts ? p.M : p.n_experts)
-                                    : (long long)(p.M + ROW_TILE - 1) / ROW_TILE;
-    const long long units = tiles * ((p.N + W_TILE - 1) / W_TILE);
+    const long long tiles = GROUPED ? (long long)(p.M / L::ROWS) + (p.M < p.n_experts ? p.M : p.n_experts)
+                                    : (long long)(p.M + L::ROWS - 1) / L::ROWS;
+    const long long units = tiles * ((p.N + NT - 1) / NT);
     if (units > 0x3fffffffLL) return MLS_ERR_UNSUPPORTED;
     const int most = sm_count() / 2, pairs = (int)(units < most ? units : most);
-    const size_t smem = L::FIXED + (GROUPED ? 4 * (p.n_experts + 1) : 0);
-    const int rc = GROUPED ? launch_plain(mx4_pair_kernel<NT, GROUPED>, dim3(2 * pairs), dim3(L::THREADS), smem, stream, p, w_map,
-                                          rows_map, sf_w_map, sf_rows_map)
-                           : launch_plain(mx4_pair_kernel<NT, GROUPED>, dim3(2 * pairs), dim3(L::THREADS), smem, stream, p,
-                                          rows_map, w_map, sf_rows_map, sf_w_map);
+    const int rc = launch_plain(mx4_pair_kernel<NT, GROUPED>, dim3(2 * pairs), dim3(L::THREADS),
+                                L::FIXED + (GROUPED ? 4 * (p.n_experts + 1) : 0), stream, p, rows_map, w_map, sf_rows_map, sf_w_map);
     return rc ? rc : launch_status();
 }
 
 // The ways of many rows, by the tile of a unit of work: 128 weights x 64 or 192 rows on one block, 256 rows x 192 or 256 weights on
-// a pair (routed: 256 weights x 256 rows).  Units are dealt out in rounds of one a block or pair; a round takes so long for every
+// a pair (routed: 256 x 256 only).  Units are dealt out in rounds of one a block or pair; a round takes so long for every
 // 256 of K, and so long for what its epilogue leaves visible (float32 sums of slots are 200 MB in a long prompt).  The
 // cheapest way is taken.  Measured, us, in the order 64 / 192 / 192 on pairs / 256 on pairs, rows quantised already:
 //   256 rows x 14,336, 4,096 outputs       21.4 / 30.3 / 21.5 / 22.5     2,048 rows          125 / 82 / 54 / 42
@@ -172,15 +166,16 @@ int launch(const Product& p, const void* rows, const void* W, cudaStream_t strea
     const double t[4] = {cost(64, 128, blocks, 0.335, 0.45, 0), cost(192, 128, blocks, of_192 > 0.345 ? of_192 : 0.345,
                                                                      0.9 + 2.5 * slots, 0),
                          GROUPED ? 1e30 : cost(256, 192, pairs, 0.355, 0.5 + 0.8 * gated, 1),
-                         GROUPED ? cost(256, 256, pairs, 0.30 + 0.0004 * rows_in(256), 0.9 + 0.6 * gated + 3 * slots, 2)
+                         GROUPED ? cost(256, 256, pairs, 0.30 + 0.0004 * rows_in(256), 0.9 + 0.6 * gated + 2 * slots, 2)
                                  : cost(256, 256, pairs, 0.365, 0.9 + 0.6 * gated, 1)};
     int best = 0;
     for (int way = 1; way < 4; ++way)
         if (t[way] < t[best]) best = way;
-    return best == 0   ? launch_nt<64, GROUPED>(p, rows, W, stream)
-           : best == 1 ? launch_nt<192, GROUPED>(p, rows, W, stream)
-           : best == 3 || GROUPED ? launch_pair<256, GROUPED>(p, rows, W, stream)
-                                  : launch_pair<(GROUPED ? 256 : 192), GROUPED>(p, rows, W, stream);
+    if (best == 0) return launch_nt<64, GROUPED>(p, rows, W, stream);
+    if (best == 1) return launch_nt<192, GROUPED>(p, rows, W, stream);
+    if constexpr (!GROUPED)
+        if (best == 2) return launch_pair<192, false>(p, rows, W, stream);
+    return launch_pair<256, GROUPED>(p, rows, W, stream);
 }
 
 template <int NR, bool FUSED>
@@ -217,7 +212,7 @@ static int product(int unit, const void* rows, int rows_type, long long ld, void
     }
     if (slice > 0) {
         const int kblocks = (K + BK - 1) / BK;
-        if (M > (fused ? 16 : 64) || (fused && slice > FEW_SLICE) || (kblocks + slice - 1) / slice > 8 ||
+        if (M > (fused ? 16 : 64) || (fused && slice > FEW_SLICE) || (kblocks + slice - 1) / slice > FEW_SLICES ||
             (w_rows + UMMA_M - 1) / UMMA_M > 65535)
             return MLS_ERR_UNSUPPORTED;
         const int vec = reinterpret_cast<uintptr_t>(rows) % 16 == 0 && ld % (rows_type == MLS_BF16 ? 8 : 4) == 0;

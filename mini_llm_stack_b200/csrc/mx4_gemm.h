@@ -243,10 +243,10 @@ __device__ __forceinline__ Rows<RUNS> rows_of(const Product& p, const Unit& u, i
     return r;
 }
 // A unit's sums on their way out: a warp takes the quarter q of the lanes (32 of the 128 rows of weights) and its set's runs of 16
-// of the batch's rows, the last first with `down`; `read(i)` is called behind the i-th one's reading.
-template <typename OUT, bool GROUPED, int RUNS, typename Read>
+// of the batch's rows.
+template <typename OUT, bool GROUPED, int RUNS>
 __device__ __forceinline__ void store_unit(const Product& p, const Unit& u, const Rows<RUNS>& rows, uint32_t tmem, int q, int set,
-                                           int sets, int lane, bool down, Read read) {
+                                           int sets, int lane) {
     const bool pairs = p.unit == GATED;
     // this thread's output
     const int n = pairs ? u.n0 / 2 + q * 16 + (lane & 15) : u.n0 + q * 32 + lane;
@@ -255,21 +255,15 @@ __device__ __forceinline__ void store_unit(const Product& p, const Unit& u, cons
     const uint32_t d = tmem + ((uint32_t)(q * 32) << 16);
 #pragma unroll
     for (int i = 0; i < RUNS; ++i) {
-        const int c0 = ((down ? RUNS - 1 - i : i) * sets + set) * 16, there = u.rows - c0;
-        if (there <= 0) {
-            read(i);
-            continue;
-        }
-        const int to = down ? rows.to[RUNS - 1 - i] : rows.to[i];
+        const int c0 = (i * sets + set) * 16, there = u.rows - c0;
+        if (there <= 0) break;
         uint32_t v[16];
         tmem_ld16(d + c0, v);
         tmem_ld_wait();
-        read(i);
         if (GROUPED && p.scale) {
 #pragma unroll
             for (int x = 0; x < 16; ++x)
-                v[x] = __float_as_uint(__uint_as_float(v[x]) *
-                                       __shfl_sync(0xffffffffu, down ? rows.share[RUNS - 1 - i] : rows.share[i], x));
+                v[x] = __float_as_uint(__uint_as_float(v[x]) * __shfl_sync(0xffffffffu, rows.share[i], x));
         }
         if (pairs) {
             // lanes 0..15 hold the gate's sums of 16 rows, lanes 16..31 up's of the same outputs: the former take the
@@ -290,7 +284,7 @@ __device__ __forceinline__ void store_unit(const Product& p, const Unit& u, cons
         } else if (GROUPED && p.unit == DOWN) {
 #pragma unroll
             for (int x = 0; x < 16; ++x) {
-                const int s = __shfl_sync(0xffffffffu, to, x);
+                const int s = __shfl_sync(0xffffffffu, rows.to[i], x);
                 if (mine && x < there) Elem<OUT>::store(out + (size_t)s * p.width, __uint_as_float(v[x]));
             }
         } else {
@@ -437,9 +431,8 @@ __device__ __forceinline__ void product_block(const Product& p, const CUtensorMa
             }
             tc_fence_after();
             const uint32_t d = tmem_base + acc * NT;
-            auto read = [](int) {};
-            if (p.out_type == MLS_BF16) store_unit<__nv_bfloat16, GROUPED, RUNS>(p, u, r, d, q, half, 2, lane, false, read);
-            else store_unit<float, GROUPED, RUNS>(p, u, r, d, q, half, 2, lane, false, read);
+            if (p.out_type == MLS_BF16) store_unit<__nv_bfloat16, GROUPED, RUNS>(p, u, r, d, q, half, 2, lane);
+            else store_unit<float, GROUPED, RUNS>(p, u, r, d, q, half, 2, lane);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(acc_empty(acc));

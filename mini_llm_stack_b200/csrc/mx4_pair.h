@@ -1,17 +1,16 @@
-// The product of many rows by pairs of blocks: two neighbouring SMs work on one tile of 256 of one operand's rows (the M side)
-// by up to NT of the other's (the N side).
+// The product of many rows by pairs of blocks: two neighbouring SMs work on one tile of 256 rows of the batch (or of an expert)
+// by up to NT rows of weights.
 //
 // At four bits a value an instruction is done with its operands in a third of the time in which L2 brings them to a lone block,
-// whose 128 x 192 tile asks for 43 KB for every 256 of K.  Here a block brings in its 128 rows of the M side and half of the N
-// side's (31 KB for 128 x 192, 35 for 128 x 256), and the instruction, issued by the first block of the pair, takes both
-// halves.  Each block holds the scales of its own M rows and of all N rows.
+// whose 128 x 192 tile asks for 43 KB for every 256 of K.  Here a block brings in its 128 rows of the batch and half of the
+// tile's weights (31 KB for 128 x 192, 35 for 128 x 256), and the instruction, issued by the first block of the pair, takes
+// both halves.  Each block holds the scales of its own rows and of all the tile's weights.
 //
-// One matrix: the batch's rows are the M side, the weights the N side.  A thread of the epilogue then holds neighbouring
-// outputs of one row, gate and up of the same output among them, and stores whole sectors of 32 bytes.  (With the weights on
-// the M side a warp's stores are 64 bytes of a row each: 2,048 rows x 28,672 x 4,096 with SwiGLU took 213 us, of which the
-// epilogue was 110.)
-// Routed: the weights are the M side, an expert's rows the N side, rounded up to 32 only: experts of a prompt have from ten to
-// some hundreds of rows, of which tiles of 256 would waste half the instructions.
+// The batch's rows lie on the 128-row side: a thread of the epilogue then holds neighbouring outputs of one row, gate and up of
+// the same output among them, and stores whole sectors of 32 bytes.  (With the weights there, a warp's stores are 64 or 128
+// bytes of a row each: 2,048 rows x 28,672 x 4,096 with SwiGLU took 213 us, of which the epilogue was 110; 2,048 tokens through 64
+// experts of 4,096 x 1,408, six chosen, 135 us down instead of 116.  Up it is no matter, 121 and 119: what tiles of 256 rows waste
+// on experts of few the wider stores win back.)
 //
 // Tensor memory: ACC_COLS columns of accumulators, every second one from the first column on, the others up to the last, so that
 // two that fit beside one another overlap: the epilogue of one lies under the instructions of the next.  NT = 192 always fits;
@@ -37,10 +36,9 @@ __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap
         : "memory");
 }
 
-template <int NT_, bool GROUPED>
+template <int NT_>
 struct PairPlan {
-    static constexpr int NT = NT_, MT = 2 * UMMA_M;
-    static constexpr int BOX = GROUPED ? 64 : NT / 2;              // N rows of a copy
+    static constexpr int NT = NT_, ROWS = 2 * UMMA_M;
     static constexpr int A_BYTES = UMMA_M * CODE_ROW, B_BYTES = NT / 2 * CODE_ROW;
     static constexpr int SF_A = A_BYTES + B_BYTES, SF_B = SF_A + SF_STAGE;
     static constexpr int STAGE = SF_B + 2 * SF_STAGE;
@@ -49,7 +47,7 @@ struct PairPlan {
     static constexpr int ACC_COLS = 384;
     static constexpr int FIT = (512 - ACC_COLS) / SF_SLOT_COLS;
     static constexpr int SF_SLOTS = FIT < STAGES ? FIT : STAGES;
-    static constexpr int SETS = GROUPED ? 4 : NT / 64;             // of four epilogue warps
+    static constexpr int SETS = NT / 64;                           // of four epilogue warps
     static constexpr int THREADS = 64 + 128 * SETS;
     static constexpr int BARS = STAGES * STAGE;                    // full, empty [STAGES]; acc_full, acc_free, acc_empty [2]
     static constexpr int TMEM_SLOT = BARS + 8 * (2 * STAGES + 6);
@@ -93,9 +91,9 @@ __device__ __forceinline__ void store_run(OUT* out, const float (&v)[COUNT], int
 
 // A warp's runs of 32 columns of the accumulator, for its 32 rows: this thread's goes to row `to`.  The set's runs lie `step`
 // columns apart, in the order in which they are to be read; `read(i)` is called behind the i-th one's reading.
-template <typename OUT, int RUNS, typename Read>
+template <typename OUT, bool GROUPED, int RUNS, typename Read>
 __device__ __forceinline__ void store_rows(const Product& p, uint32_t d, int set, int sets, bool down, int columns, int n0,
-                                           bool any, bool mine, int to, bool vec, Read read) {
+                                           bool any, bool mine, int to, float share, bool vec, Read read) {
     OUT* row = (OUT*)p.out + (size_t)to * p.width;
     const bool pairs = p.unit == GATED, square = p.unit == RELU2;
 #pragma unroll 1
@@ -114,7 +112,9 @@ __device__ __forceinline__ void store_rows(const Product& p, uint32_t d, int set
             float v[16];
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
-                v[j] = unit_of_sums<OUT>(__uint_as_float(x[j]), __uint_as_float(y[j]), p.alpha, p.limit);
+                float g = __uint_as_float(x[j]), up = __uint_as_float(y[j]);
+                if (GROUPED) g *= share, up *= share;
+                v[j] = unit_of_sums<OUT>(g, up, p.alpha, p.limit);
             }
             const int col = (n0 + c0) / 2;
             if (mine) store_run<OUT>(row + col, v, p.width - col, vec);
@@ -123,6 +123,7 @@ __device__ __forceinline__ void store_rows(const Product& p, uint32_t d, int set
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
                 v[j] = __uint_as_float(j < 16 ? x[j & 15] : y[j & 15]);
+                if (GROUPED) v[j] *= share;
                 if (square) v[j] = fmaxf(v[j], 0.f) * fmaxf(v[j], 0.f);
             }
             const int col = n0 + c0;
@@ -131,12 +132,10 @@ __device__ __forceinline__ void store_rows(const Product& p, uint32_t d, int set
     }
 }
 
-// m_map, n_map: codes of the operands; sf_m_map, sf_n_map: their scales.
 template <int NT_, bool GROUPED>
-__device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* m_map, const CUtensorMap* n_map,
-                                           const CUtensorMap* sf_m_map, const CUtensorMap* sf_n_map) {
-    using L = PairPlan<NT_, GROUPED>;
-    constexpr int ROW_TILE = GROUPED ? L::NT : L::MT, W_TILE = GROUPED ? L::MT : L::NT;
+__device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* rows_map, const CUtensorMap* w_map,
+                                           const CUtensorMap* sf_rows_map, const CUtensorMap* sf_w_map) {
+    using L = PairPlan<NT_>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
     const uint32_t base = (raw + 1023u) & ~1023u;
@@ -168,19 +167,19 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
         chain_release();                 // (not before: see there)
     }
     chain_wait();
-    if (GROUPED && warp == 0) row_tiles<ROW_TILE>(p, lane, start);
+    if (GROUPED && warp == 0) row_tiles<L::ROWS>(p, lane, start);
     tc_fence_before();
     __syncwarp();
     cluster_sync_all();                  // both blocks' barriers, tables and tensor memory are ready
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
-    const int w_tiles = (p.N + W_TILE - 1) / W_TILE, sf_tiles = (p.N + TILE_ROWS - 1) / TILE_ROWS;
-    const int units = (GROUPED ? start[p.n_experts] : (p.M + ROW_TILE - 1) / ROW_TILE) * w_tiles;
+    const int w_tiles = (p.N + L::NT - 1) / L::NT, sf_tiles = (p.N + TILE_ROWS - 1) / TILE_ROWS;
+    const int units = (GROUPED ? start[p.n_experts] : (p.M + L::ROWS - 1) / L::ROWS) * w_tiles;
     const int kblocks = (p.K + BK - 1) / BK;
     const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
     bool timed_out = false;
-    // the accumulator's columns, up to a multiple of 32 (a half of the N rows comes from each block), and where they are
-    auto columns = [&](const Unit& u) { return ((GROUPED ? u.rows : min(L::NT, p.N - u.n0)) + 31) & ~31; };
+    // the accumulator's columns, up to a multiple of 32 (a half of the weights comes from each block), and where they are
+    auto columns = [&](const Unit& u) { return (min(L::NT, p.N - u.n0) + 31) & ~31; };
     auto place = [&](const Unit& u, int it) { return it & 1 ? L::ACC_COLS - columns(u) : 0; };
 
     if (warp == 0) {
@@ -188,27 +187,25 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
         if (lane == 0) {
             int g = 0;
             for (int i = first; i < units && !timed_out; i += step) {
-                const Unit u = unit_of<ROW_TILE, GROUPED, W_TILE>(p, i, w_tiles, start);
-                const int half = columns(u) / 2, boxes = GROUPED ? (half + L::BOX - 1) / L::BOX : 1;
-                const uint32_t bytes = 2 * (L::A_BYTES + boxes * (L::BOX * CODE_ROW) + 3 * SF_STAGE);
-                const int w_row = u.e * p.N + u.n0, sf_w = u.e * sf_tiles + u.n0 / TILE_ROWS;
-                const int m_row = (GROUPED ? w_row : u.row0) + (int)rank * UMMA_M;
-                const int n_row = (GROUPED ? u.row0 : w_row) + (int)rank * half;
-                const int sf_m = (GROUPED ? sf_w : u.sf_tile) + (int)rank, sf_n = GROUPED ? u.sf_tile : sf_w;
+                const Unit u = unit_of<L::ROWS, GROUPED, L::NT>(p, i, w_tiles, start);
+                // (a second block without rows brings in none)
+                const bool second = u.rows > UMMA_M, with_rows = rank == 0 || second;
+                const uint32_t bytes = (second ? 2 : 1) * L::A_BYTES + 2 * (L::B_BYTES + 3 * SF_STAGE);
+                const int row = u.row0 + (int)rank * UMMA_M, w_row = u.e * p.N + u.n0 + (int)rank * (columns(u) / 2);
+                const int sf_row = u.sf_tile + (int)rank, sf_w = u.e * sf_tiles + u.n0 / TILE_ROWS;
                 for (int kb = 0; kb < kblocks; ++kb, ++g) {
                     const int slot = g % L::STAGES;
                     if (!mbar_wait(empty(slot), ((g / L::STAGES) & 1) ^ 1)) {
                         timed_out = true;
                         break;
                     }
-                    const uint32_t a = base + slot * L::STAGE, b = a + L::A_BYTES, bar = full(slot);
+                    const uint32_t a = base + slot * L::STAGE, bar = full(slot);
                     // both blocks' copies of the stage complete on the first one's barrier
                     if (rank == 0) mbar_arrive_expect_tx(bar, bytes);
-                    tma_load_2d_pair(a, m_map, kb * CODE_ROW, m_row, bar);
-                    for (int x = 0; x < boxes; ++x)
-                        tma_load_2d_pair(b + x * (L::BOX * CODE_ROW), n_map, kb * CODE_ROW, n_row + x * L::BOX, bar);
-                    tma_load_3d_pair(a + L::SF_A, sf_m_map, 0, kb, sf_m, bar);
-                    tma_load_3d_pair(a + L::SF_B, sf_n_map, 0, kb, sf_n, bar);
+                    if (with_rows) tma_load_2d_pair(a, rows_map, kb * CODE_ROW, row, bar);
+                    tma_load_2d_pair(a + L::A_BYTES, w_map, kb * CODE_ROW, w_row, bar);
+                    tma_load_3d_pair(a + L::SF_A, sf_rows_map, 0, kb, sf_row, bar);
+                    tma_load_3d_pair(a + L::SF_B, sf_w_map, 0, kb, sf_w, bar);
                 }
             }
             // the copies under way land before the pair's shared memory goes away (the first block's barriers count both
@@ -227,7 +224,7 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
             int it = 0, columns_before = 0, slot = 0, phase = 0;
             int sf_slot = 0, old = L::STAGES - L::SF_SLOTS, old_phase = 1;      // (the phase before the first is over)
             for (int i = first; i < units && !timed_out; i += step, ++it) {
-                const Unit u = unit_of<ROW_TILE, GROUPED, W_TILE>(p, i, w_tiles, start);
+                const Unit u = unit_of<L::ROWS, GROUPED, L::NT>(p, i, w_tiles, start);
                 const int n = columns(u), acc = it & 1;
                 const uint32_t idesc0 = idesc_mx4(2 * UMMA_M, n, 0), idesc1 = idesc_mx4(2 * UMMA_M, n, 1);
                 // the accumulator before the last has been read, and of the last the columns that this one may take, where
@@ -239,7 +236,7 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
                     break;
                 }
                 columns_before = n;
-                const uint32_t d = tmem_base + place(u, it), shift = (GROUPED ? u.sf_row : u.n0 % TILE_ROWS) / 32;
+                const uint32_t d = tmem_base + place(u, it), shift = u.n0 % TILE_ROWS / 32;
                 int left = p.K;
                 for (int kb = 0; kb < kblocks; ++kb, left -= BK) {
                     // the stage is there, and the instructions that read its scales' columns last are done: both asked at
@@ -272,8 +269,8 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
     } else {
         // -------------------------------------------------------------------- epilogue
         const int q = warp & 3, set = (warp - 2) >> 2;
-        // runs of 16 (routed) or 32 columns a set: two or more, the first half of them in the columns that the next may take
-        constexpr int RUNS = L::NT / (GROUPED ? 16 : 32) / L::SETS, FREE_AT = L::NT == 256 ? RUNS / 2 - 1 : RUNS - 1;
+        // two runs of 32 columns a set: the first of 256 in the columns that the next accumulator may take
+        constexpr int RUNS = L::NT / 32 / L::SETS, FREE_AT = L::NT == 256 ? RUNS / 2 - 1 : RUNS - 1;
         const bool vec = p.width % (p.out_type == MLS_BF16 ? 16 : 8) == 0 && reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
         auto arrive = [&](uint32_t bar) {
             tc_fence_before();
@@ -285,7 +282,7 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
         };
         int it = 0;
         for (int i = first; i < units; i += step, ++it) {
-            Unit u = unit_of<ROW_TILE, GROUPED, W_TILE>(p, i, w_tiles, start);
+            const Unit u = unit_of<L::ROWS, GROUPED, L::NT>(p, i, w_tiles, start);
             const int acc = it & 1;
             // (the columns in the middle first: an accumulator at the end begins there, one at the start ends there)
             const bool down = acc == 0;
@@ -294,26 +291,27 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
                 if (run == FREE_AT) arrive(acc_free(acc));
                 if (run == RUNS - 1) arrive(acc_empty(acc));
             };
-            Rows<RUNS> r;
-            if (GROUPED) r = rows_of<GROUPED, RUNS>(p, u, set, L::SETS, lane);
+            // where this thread's row goes and the weight of its slot, read while the instructions still run
+            const int row = (int)rank * UMMA_M + q * 32;
+            const bool any = row < u.rows, mine = row + lane < u.rows;
+            int to = u.row0 + row + lane;
+            float share = 1.f;
+            if (GROUPED && mine && (p.unit == DOWN || p.scale)) {
+                const int s = p.order[to];
+                if (p.scale) share = p.weight[s];
+                if (p.unit == DOWN) to = s;
+            }
             if (!mbar_wait_warp(acc_full(acc), (it >> 1) & 1)) {
                 timed_out = true;
                 break;
             }
             tc_fence_after();
-            if constexpr (GROUPED) {
-                u.n0 += (int)rank * UMMA_M;
-                if (p.out_type == MLS_BF16) store_unit<__nv_bfloat16, GROUPED, RUNS>(p, u, r, d, q, set, L::SETS, lane, down, read);
-                else store_unit<float, GROUPED, RUNS>(p, u, r, d, q, set, L::SETS, lane, down, read);
-            } else {
-                const int row = (int)rank * UMMA_M + q * 32 + lane;
-                const uint32_t at = d + ((uint32_t)(q * 32) << 16);
-                const bool any = (int)rank * UMMA_M + q * 32 < u.rows, mine = row < u.rows;
-                if (p.out_type == MLS_BF16)
-                    store_rows<__nv_bfloat16, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, mine, u.row0 + row, vec, read);
-                else
-                    store_rows<float, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, mine, u.row0 + row, vec, read);
-            }
+            const uint32_t at = d + ((uint32_t)(q * 32) << 16);
+            if (p.out_type == MLS_BF16)
+                store_rows<__nv_bfloat16, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, mine, to, share, vec,
+                                                         read);
+            else
+                store_rows<float, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, mine, to, share, vec, read);
         }
     }
     if (timed_out && p.status) atomicOr(p.status, MLS_STATUS_TIMEOUT);

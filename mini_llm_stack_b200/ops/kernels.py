@@ -125,30 +125,30 @@ class Mx4:
     0.5, 1, 1.5, 2, 3, 4, 6.  ``codes``: uint8 ``[all rows, bytes]``, two codes a byte, the even place in the low bits;
     ``scales``: uint8 ``[tiles, atoms, 512]`` in the order in which they enter the tensor cores (csrc/mx4.h)."""
 
-    __slots__ = ("shape", "gate_up", "data", "lead", "n", "k", "rows", "tiles", "scales_at", "codes_at", "slice", "settled")
+    __slots__ = ("shape", "gate_up", "data", "lead", "n", "k", "rows", "tiles", "scales_at", "codes_at", "settled", "_slice")
     TILE_ROWS = 128
 
-    def __init__(self, shape, device, gate_up: bool = False, sm_count: int = 148):
+    def __init__(self, shape, device, gate_up: bool = False):
         """Memory for matrices of this shape; ``gate_up``: pairs ``[..., 2, N, K]`` of a gate and an up matrix whose
         rows lie interleaved, 16 and 16."""
-        self.shape, self.gate_up = tuple(shape), gate_up
-        *lead, n, k = self.shape
+        shape = tuple(shape)
+        n, k = shape[-2:]
         mats = 1
-        for i in lead:
+        for i in shape[:-2]:
             mats *= i
-        self.lead = len(lead) - gate_up              # dimensions in front of a matrix or a pair
-        self.n, self.k = n, k
+        self.shape, self.gate_up, self.n, self.k = shape, gate_up, n, k
+        self.lead = len(shape) - 2 - gate_up         # dimensions in front of a matrix or a pair
         if gate_up:
-            mats, n = mats // 2, -(-n // 16) * 32
-        self.rows, self.tiles = mats * n, mats * -(-n // 128)
-        room = self.tiles * self.tile_bytes(k) + self.rows * self.pitch(k)
+            mats, n = mats // 2, (n + 15) // 16 * 32
+        self.rows, self.tiles = mats * n, mats * ((n + 127) // 128)
+        scales = self.tiles * self.tile_bytes(k)
         # (what fills up a pair's rows is read, so it is zeroed)
         new = torch.zeros if gate_up and n != 2 * self.n else torch.empty
-        self.data = new(room, dtype=torch.uint8, device=device)
+        self.data = new(scales + self.rows * self.pitch(k), dtype=torch.uint8, device=device)
         self.scales_at = self.data.data_ptr()
-        self.codes_at = self.scales_at + self.tiles * self.tile_bytes(k)
-        self.slice = self._few_rows_slice(sm_count, n, k)
+        self.codes_at = self.scales_at + scales
         self.settled = False          # whether the device has finished what wrote it
+        self._slice = None
 
     @staticmethod
     def pitch(k: int) -> int:
@@ -160,15 +160,17 @@ class Mx4:
         """Bytes of scales of 128 rows."""
         return (k + 255) // 256 * 1024
 
-    def _few_rows_slice(self, sm_count: int, n: int, k: int) -> int:
+    def few_rows_slice(self, sm_count: int) -> int:
         """How much of K, in steps of 256, a block of the product of few rows takes: as many slices, up to eight, as leave
         all blocks resident at once, two an SM (a block that comes in a second round costs more than its slice saves).
         0: the tiles alone are more, the product takes the way of many rows.  (In us, this way and that one: 8 rows, 4,096
         outputs of 14,336 in eight slices 9.3 and 20.8, 28,672 of 4,096 in one 14.4 and 17.5.  From 17 rows on one or two slices
         do not pay: 32 rows, 28,672 of 4,096 16.9 and 16.3, 7,168 of 4,096 in four slices 8.4 and 9.3.)"""
-        steps, tiles = -(-k // 256), max(1, -(-n // 128))
-        slices = min(8, steps, 2 * sm_count * 19 // 20 // tiles)
-        return -(-steps // slices) if slices else 0
+        if self._slice is None:
+            steps, tiles = -(-self.k // 256), max(1, self.tiles)
+            slices = min(8, steps, 2 * sm_count * 19 // 20 // tiles)
+            self._slice = -(-steps // slices) if slices else 0
+        return self._slice
 
     @property
     def codes(self):
@@ -1472,18 +1474,22 @@ class Ops:
     MX4_ONCE = 1 << 16       # slots x steps of 256 of K from which on tokens are quantised once
     MX4_FUSED_TASKS = 64     # 256 values of a row each: with so many a block the product quantises its rows itself
 
+    def _mx4(self, name: str):
+        fns = self._part_libs.get("mx4")
+        return (fns or self._part_lib("mx4"))[name]
+
     def _mx4_here(self, what: str, *tensors) -> None:
+        here = self._device_index
         for t in tensors:
-            if t.get_device() != self._device_index:
+            if t.get_device() != here:
                 raise KernelError(f"{what}: tensors must be on {self.device}")
-        if _current_device() != self._device_index:
+        if _current_device() != here:
             raise KernelError(f"{what}: {self.device} must be the current device")
 
     @staticmethod
-    def _mx4_apart(rows, ld: int, out, what: str) -> None:
+    def _mx4_apart(rows: int, row_bytes: int, out: int, out_bytes: int, what: str) -> None:
         """A product's blocks read rows while others store outputs already."""
-        a, b, (m, k) = rows.data_ptr(), out.data_ptr(), rows.shape
-        if a < b + out.numel() * out.element_size() and b < a + ((m - 1) * ld + k) * rows.element_size():
+        if rows < out + out_bytes and out < rows + row_bytes:
             raise KernelError(f"{what}: the output lies where the rows are")
 
     @staticmethod
@@ -1497,9 +1503,11 @@ class Ops:
     def _mx4_ld(x, k: int, what: str) -> int:
         """The distance of a matrix's rows, whose values must lie side by side."""
         ld, step = x.stride()
-        if (step != 1 and k > 1) or (ld < k and x.shape[0] > 1):
+        if ld >= k and step == 1:
+            return ld
+        if (step != 1 and k > 1) or x.shape[0] > 1:
             raise KernelError(f"{what}: a row's values must lie side by side, rows must not overlap")
-        return ld if ld > k else k
+        return k
 
     def quantize_mx4(self, x, into: Mx4 | None = None, gate_up: bool = False) -> Mx4:
         """The rows of ``x [..., rows, K]`` (float32 or bfloat16; two-dimensional ones may have a row stride) as 4-bit
@@ -1516,8 +1524,9 @@ class Ops:
         if len(shape) < 2 or not 1 <= shape[-1] <= self.MX4_MOST_K or x.numel() // shape[-1] > self.MX4_MOST_ROWS:
             raise KernelError(f"{what}: matrices [..., rows, K] with K from 1 to {self.MX4_MOST_K} and at most "
                               f"{self.MX4_MOST_ROWS} rows, not {shape}")
-        if gate_up and (len(shape) < 3 or shape[-3] != 2):
-            raise KernelError(f"{what}: gate_up goes with matrices [..., 2, N, K], not {shape}")
+        if gate_up and (len(shape) < 3 or shape[-3] != 2 or x.numel() // shape[-1] * 16 > self.MX4_MOST_ROWS * shape[-2]):
+            raise KernelError(f"{what}: gate_up goes with matrices [..., 2, N, K], at most {self.MX4_MOST_ROWS} rows with each "
+                              f"matrix filled up to 16, not {shape}")
         self._mx4_here(what, x)
         k = shape[-1]
         if len(shape) == 2:
@@ -1527,7 +1536,7 @@ class Ops:
             ld, rows = k, x.numel() // k
         gate_up = bool(gate_up)
         if into is None:
-            into = Mx4(shape, x.device, gate_up, self.sm_count)
+            into = Mx4(shape, x.device, gate_up)
         elif into.__class__ is not Mx4 or into.shape != shape or into.gate_up != gate_up:
             raise KernelError(f"{what}: into is laid out for something else")
         else:
@@ -1535,8 +1544,8 @@ class Ops:
             into.settled = False
         if rows:
             self.launches += 1
-            rc = self._part_lib("mx4")["quantize"](x.data_ptr(), code, ld, rows, k, shape[-2], gate_up, into.codes_at,
-                                                   into.scales_at, self._stream())
+            rc = self._mx4("quantize")(x.data_ptr(), code, ld, rows, k, shape[-2], gate_up, into.codes_at, into.scales_at,
+                                       self._stream())
             if rc:
                 _check(rc, what)
         return into
@@ -1551,8 +1560,7 @@ class Ops:
         rows = out.numel() // q.k
         if rows:
             self.launches += 1
-            rc = self._part_lib("mx4")["values"](q.codes_at, q.scales_at, rows, q.k, q.n, q.gate_up, out.data_ptr(), code,
-                                                 self._stream())
+            rc = self._mx4("values")(q.codes_at, q.scales_at, rows, q.k, q.n, q.gate_up, out.data_ptr(), code, self._stream())
             if rc:
                 _check(rc, what)
 
@@ -1598,7 +1606,10 @@ class Ops:
             return
         rows = codes = scales = None
         code, ld, fused = -1, 0, False
-        few = w.slice
+        few = w._slice
+        if few is None:
+            few = w.few_rows_slice(self.sm_count)
+        to = out.data_ptr()
         if m > 16 and (m > 64 or 4 * few > -(-k // 256)):
             few = 0
         if ready:
@@ -1607,15 +1618,14 @@ class Ops:
             codes, scales = a.codes_at, a.scales_at
         else:
             code, ld, rows = self._mx4_type(a, what), self._mx4_ld(a, k, what), a.data_ptr()
-            self._mx4_apart(a, ld, out, what)
+            self._mx4_apart(rows, ((m - 1) * ld + k) * (4 - 2 * code), to, m * n * (4 - 2 * out_type), what)
             fused = 0 < few <= 12 and m <= 16 and m * few <= self.MX4_FUSED_TASKS
             if not fused:
                 codes, scales, _, _ = self._mx4_scratch(m, k, (m + 127) // 128)
                 self.launches += 1
         self.launches += 1
-        rc = self._part_lib("mx4")["product"](unit, rows, code, ld, codes, scales, w.codes_at, w.scales_at, out.data_ptr(),
-                                              out_type, m, n, k, few, fused, w.settled, alpha, limit, self._status_at,
-                                              self._stream())
+        rc = self._mx4("product")(unit, rows, code, ld, codes, scales, w.codes_at, w.scales_at, to, out_type, m, n, k, few, fused,
+                                  w.settled, alpha, limit, self._status_at, self._stream())
         if rc:
             _check(rc, what)
 
@@ -1658,14 +1668,15 @@ class Ops:
             return
         if slots > self.MX4_MOST_ROWS:
             raise KernelError(f"{what}: at most {self.MX4_MOST_ROWS} slots")
-        self._mx4_apart(rows, ld, out, what)
+        at, to = rows.data_ptr(), out.data_ptr()
+        self._mx4_apart(at, ((shape[0] - 1) * ld + k) * (4 - 2 * code), to, slots * n * (4 - 2 * out_type), what)
         # (many slots: every token is quantised once and copied to its slots; 12,288 slots of 2,048 tokens x 4,096 in 12 us
         # where they took 27 one by one)
         tokens = shape[0] if unit and top > 1 and slots * -(-k // 256) >= self.MX4_ONCE else 0
         codes, scales, t_codes, t_scales = self._mx4_scratch(slots, k, slots // 128 + n_experts + 1, tokens)
         self.launches += (2 if tokens else 1) - (-n_experts // 1024)
-        rc = self._part_lib("mx4")["expert_product"](
-            unit, rows.data_ptr(), code, ld, top, unit != 0, tokens, t_codes, t_scales, codes, scales, w.codes_at, w.scales_at, out.data_ptr(), out_type,
+        rc = self._mx4("expert_product")(
+            unit, at, code, ld, top, unit != 0, tokens, t_codes, t_scales, codes, scales, w.codes_at, w.scales_at, to, out_type,
             slots, n_experts, n, k, order.data_ptr(), idx.data_ptr(), offsets.data_ptr(), weight.data_ptr(), scale, alpha,
             limit, self._status_at, self._stream())
         if rc:

@@ -11,7 +11,7 @@ from mini_llm_stack_b200.ops.kernels import KernelError, Mx4, Ops
 def ops():
     """The checks of the kernels' owner without a device: tensors of the CPU pass for its own."""
     o = Ops.__new__(Ops)
-    o.device, o._device_index, o.sm_count, o.launches = torch.device("cpu"), -1, 148, 0
+    o.device, o._device_index, o.sm_count, o.launches, o._part_libs = torch.device("cpu"), -1, 148, 0, {}
 
     def here(what, *tensors):
         assert all(isinstance(t, torch.Tensor) for t in tensors)
@@ -37,7 +37,7 @@ def test_sizes_in_memory():
                                   (256, 1 << 20)])
 def test_slices_are_eight_at_most_and_resident_at_once(n, k):
     steps, tiles = -(-k // 256), -(-n // 128)
-    s = Mx4((n, k), "meta").slice if n * k > 1 << 24 else Mx4((n, k), "cpu").slice
+    s = Mx4((n, k), "meta" if n * k > 1 << 24 else "cpu").few_rows_slice(148)
     if s == 0:
         assert tiles > 281
     else:
@@ -54,6 +54,8 @@ def test_rows_that_are_refused(ops):
             ops.quantize_mx4(x)
     with pytest.raises(KernelError):
         ops.quantize_mx4(torch.zeros(3, 4, 8), gate_up=True)
+    with pytest.raises(KernelError):
+        ops.quantize_mx4(torch.zeros(1).expand(1 << 24, 2, 1, 1), gate_up=True)
     for into in (Mx4((3, 4), "cpu"), Mx4((2, 4, 8), "cpu"), torch.zeros(2, 4, 8)):
         with pytest.raises(KernelError):
             ops.quantize_mx4(torch.zeros(2, 4, 8), into=into, gate_up=True)
