@@ -32,12 +32,26 @@ mx4_quantize_kernel(const T* __restrict__ x, long long ld, const Tasks tasks, in
     unsigned p = first / tasks.chunks, chunk = first - p * tasks.chunks;
     Eight<T> held[UNROLL];
     unsigned row[UNROLL], at[UNROLL];
+    int slot[UNROLL], e[UNROLL], o[UNROLL];
+    // (a slot's number, its expert and that one's first row: loads that wait for one another, but for no other task's)
+    if (map.offsets) {
+        unsigned p1 = p, c1 = chunk;
+#pragma unroll
+        for (int j = 0; j < UNROLL; ++j) {
+            row[j] = p1;
+            slot[j] = p1 < tasks.rows ? map.order[p1] : 0;
+            tasks.next(p1, c1);
+        }
+#pragma unroll
+        for (int j = 0; j < UNROLL; ++j) e[j] = row[j] < tasks.rows ? map.idx[slot[j]] : 0;
+#pragma unroll
+        for (int j = 0; j < UNROLL; ++j) o[j] = row[j] < tasks.rows && e[j] < map.n_experts ? map.offsets[e[j]] : 0;
+    }
 #pragma unroll
     for (int j = 0; j < UNROLL; ++j) {
         row[j] = p, at[j] = chunk;
         if (p < tasks.rows) {
-            unsigned from = p;
-            if (map.gather) from = (unsigned)(map.order[p] / map.top);
+            const unsigned from = map.gather ? (unsigned)(slot[j] / map.top) : p;
             held[j] = load8<T, VEC>(x + (long long)from * ld, (int)chunk * 256 + lane * 8, K);
         }
         tasks.next(p, chunk);
@@ -49,11 +63,9 @@ mx4_quantize_kernel(const T* __restrict__ x, long long ld, const Tasks tasks, in
         const uint32_t packed = quantize8(held[j], lane, word);
         Place to;
         if (map.offsets) {
-            const int e = map.idx[map.order[row[j]]];
-            if (e >= map.n_experts) continue;       // a slot of an output without weights: nobody reads it
-            const int o = map.offsets[e];
-            const unsigned r = row[j] - o;
-            to = {row[j], first_tile(o, e) + r / TILE_ROWS, r % TILE_ROWS};
+            if (e[j] >= map.n_experts) continue;    // a slot of an output without weights: nobody reads it
+            const unsigned r = row[j] - o[j];
+            to = {row[j], first_tile(o[j], e[j]) + r / TILE_ROWS, r % TILE_ROWS};
         } else {
             to = place_of(row[j], map.rows_per_mat, map.pairs);
         }
