@@ -1,18 +1,20 @@
 // Rows to 4-bit microscaled floating point (mx4.h) and back.
 //
-// Eight values a thread, four threads a block, a warp 256 of a row: 16 or 32 bytes a load, 4 bytes of codes a store,
-// the four scales of 128 values as one word.  What bounds it: the rows are read once and a quarter (or an eighth) of
-// that is written; 14,336 x 4,096 float32 values in 40.8 us (6.5 TB/s), bfloat16 in 31.6 (4.7 TB/s: some forty
-// instructions for 8 values of 16 bits).  Back to float32 43.4 us, to bfloat16 26.4.
+// Sixteen values a thread, two threads a block, a warp 512 of a row: 8 bytes of codes a store, the four scales of 128 values
+// as one word (eight values a thread: 33.9 us for 14,336 x 4,096 bfloat16 values instead of 25.3, most of it what a task
+// costs beside its values).  What bounds it: the rows are read once and a quarter (or an eighth) of that is written; 14,336 x
+// 4,096 float32 values in 39.5 us (6.7 TB/s), bfloat16 in 25.3 (5.9 TB/s, the instructions beside the loads).  Back to
+// float32 43.3 us, to bfloat16 26.3.
 #include "mx4.h"
 #include <type_traits>
 
 namespace {
 using namespace mls_mx4;
 
-// A warp's task: 256 values of a row.  Tasks are numbered along the rows; a warp takes UNROLL of them, as many apart as there
+// A warp's task: PART values of a row.  Tasks are numbered along the rows; a warp takes UNROLL of them, as many apart as there
 // are warps, whose loads are under way together.
-constexpr int UNROLL = 4;
+constexpr int UNROLL = 4, PART_VALUES = 256;                       // of values read back
+constexpr int QUANTIZE_UNROLL = 2, QUANTIZE_PART = 512;           // of values quantised
 struct Tasks {
     unsigned rows, chunks, step_row, step_chunk;
     __device__ __forceinline__ void next(unsigned& row, unsigned& chunk) const {
@@ -27,40 +29,42 @@ mx4_quantize_kernel(const T* __restrict__ x, long long ld, const Tasks tasks, in
                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     chain_release();
     chain_wait();
-    const int pitch = pitch_of(K), lane = threadIdx.x & 31;
+    const int pitch = pitch_of(K), atoms = atoms_of(K), lane = threadIdx.x & 31;
     const unsigned first = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     unsigned p = first / tasks.chunks, chunk = first - p * tasks.chunks;
-    Eight<T> held[UNROLL];
-    unsigned row[UNROLL], at[UNROLL];
-    int slot[UNROLL], e[UNROLL], o[UNROLL];
+    Eight<T> held[QUANTIZE_UNROLL][2];
+    unsigned row[QUANTIZE_UNROLL], at[QUANTIZE_UNROLL];
+    int slot[QUANTIZE_UNROLL], e[QUANTIZE_UNROLL], o[QUANTIZE_UNROLL];
     // (a slot's number, its expert and that one's first row: loads that wait for one another, but for no other task's)
     if (map.offsets) {
         unsigned p1 = p, c1 = chunk;
 #pragma unroll
-        for (int j = 0; j < UNROLL; ++j) {
+        for (int j = 0; j < QUANTIZE_UNROLL; ++j) {
             row[j] = p1;
             slot[j] = p1 < tasks.rows ? map.order[p1] : 0;
             tasks.next(p1, c1);
         }
 #pragma unroll
-        for (int j = 0; j < UNROLL; ++j) e[j] = row[j] < tasks.rows ? map.idx[slot[j]] : 0;
+        for (int j = 0; j < QUANTIZE_UNROLL; ++j) e[j] = row[j] < tasks.rows ? map.idx[slot[j]] : 0;
 #pragma unroll
-        for (int j = 0; j < UNROLL; ++j) o[j] = row[j] < tasks.rows && e[j] < map.n_experts ? map.offsets[e[j]] : 0;
+        for (int j = 0; j < QUANTIZE_UNROLL; ++j) o[j] = row[j] < tasks.rows && e[j] < map.n_experts ? map.offsets[e[j]] : 0;
     }
 #pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
+    for (int j = 0; j < QUANTIZE_UNROLL; ++j) {
         row[j] = p, at[j] = chunk;
         if (p < tasks.rows) {
             const unsigned from = map.gather ? (unsigned)(slot[j] / map.top) : p;
-            held[j] = load8<T, VEC>(x + (long long)from * ld, (int)chunk * 256 + lane * 8, K);
+            const int k0 = (int)chunk * QUANTIZE_PART + lane * 16;
+            held[j][0] = load8<T, VEC>(x + (long long)from * ld, k0, K);
+            held[j][1] = load8<T, VEC>(x + (long long)from * ld, k0 + 8, K);
         }
         tasks.next(p, chunk);
     }
 #pragma unroll
-    for (int j = 0; j < UNROLL; ++j) {
+    for (int j = 0; j < QUANTIZE_UNROLL; ++j) {
         if (row[j] >= tasks.rows) break;
-        uint32_t word;
-        const uint32_t packed = quantize8(held[j], lane, word);
+        uint32_t word, packed[2];
+        quantize_lane(held[j], lane, packed, word);
         Place to;
         if (map.offsets) {
             if (e[j] >= map.n_experts) continue;    // a slot of an output without weights: nobody reads it
@@ -69,11 +73,11 @@ mx4_quantize_kernel(const T* __restrict__ x, long long ld, const Tasks tasks, in
         } else {
             to = place_of(row[j], map.rows_per_mat, map.pairs);
         }
-        const int byte = (int)at[j] * 128 + lane * 4;              // of the row's
-        if (byte < pitch) *reinterpret_cast<uint32_t*>(codes + (size_t)to.row * pitch + byte) = packed;
-        if ((lane & 15) == 0)
-            *reinterpret_cast<uint32_t*>(scales + (((size_t)to.tile * tasks.chunks + at[j]) * 2 + (lane >> 4)) * ATOM +
-                                         row_in_atom(to.r)) = word;
+        const int byte = (int)at[j] * (QUANTIZE_PART / 2) + lane * 8, atom = (int)at[j] * 4 + (lane >> 3);
+        if (byte < pitch)
+            *reinterpret_cast<uint2*>(codes + (size_t)to.row * pitch + byte) = make_uint2(packed[0], packed[1]);
+        if ((lane & 7) == 0 && atom < atoms)
+            *reinterpret_cast<uint32_t*>(scales + ((size_t)to.tile * atoms + atom) * ATOM + row_in_atom(to.r)) = word;
     }
 }
 
@@ -170,10 +174,10 @@ mx4_values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 // The tasks and the blocks of eight warps for them; false: more tasks than a launch numbers.
-bool tasks_of(long long rows, int K, Tasks& tasks, unsigned& blocks) {
-    const long long chunks = (K + 255) / 256, n = rows * chunks;
+bool tasks_of(long long rows, int K, int part, int unroll, Tasks& tasks, unsigned& blocks) {
+    const long long chunks = (K + part - 1) / part, n = rows * chunks;
     if (n > 0x7fffffffLL) return false;
-    blocks = (unsigned)((n + 8 * UNROLL - 1) / (8 * UNROLL));
+    blocks = (unsigned)((n + 8 * unroll - 1) / (8 * unroll));
     // (few tasks: a warp each, as long as the SMs have room for them)
     const unsigned room = 4u * (unsigned)sm_count(), each = (unsigned)((n + 7) / 8);
     if (blocks < room) blocks = each < room ? each : room;
@@ -187,7 +191,7 @@ int quantize(const void* x, long long ld, long long rows, int K, const RowMap& m
              bool chained, cudaStream_t stream) {
     Tasks tasks;
     unsigned blocks;
-    if (!tasks_of(rows, K, tasks, blocks)) return MLS_ERR_UNSUPPORTED;
+    if (!tasks_of(rows, K, QUANTIZE_PART, QUANTIZE_UNROLL, tasks, blocks)) return MLS_ERR_UNSUPPORTED;
     auto* kernel = aligned16(x) && ld % (16 / (int)sizeof(T)) == 0 ? mx4_quantize_kernel<T, true> : mx4_quantize_kernel<T, false>;
     const int rc = chained ? launch_chained(kernel, dim3(blocks), dim3(256), 0, stream, (const T*)x, ld, tasks, K, map, codes, scales)
                            : launch_plain(kernel, dim3(blocks), dim3(256), 0, stream, (const T*)x, ld, tasks, K, map, codes, scales);
@@ -224,7 +228,7 @@ MLS_API int mls_mx4_values(const void* codes, const void* scales, long long rows
     if (K <= 0 || rows_per_mat <= 0) return MLS_ERR_UNSUPPORTED;
     Tasks tasks;
     unsigned blocks;
-    if (!tasks_of(rows, K, tasks, blocks)) return MLS_ERR_UNSUPPORTED;
+    if (!tasks_of(rows, K, PART_VALUES, UNROLL, tasks, blocks)) return MLS_ERR_UNSUPPORTED;
     const bool vec = K % (dtype == MLS_BF16 ? 8 : 4) == 0 && aligned16(out);
     if (dtype == MLS_BF16)
         MLS_LAUNCH((mx4_values_kernel<__nv_bfloat16>), dim3(blocks), dim3(256), 0, (cudaStream_t)stream,

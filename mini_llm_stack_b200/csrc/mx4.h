@@ -157,7 +157,7 @@ __device__ __forceinline__ float max_abs(float a, float b, float c) {
     return m;
 }
 
-// A lane's eight of a warp's 256 neighbouring values as codes; four lanes share a block.  `scales` is, in lanes 0 and 16, the
+// A lane's 8 EIGHTS neighbouring values as codes; 4 / EIGHTS lanes share a block.  `scales` is, in every (16 / EIGHTS)th lane, the
 // four scales of the 128 values from that lane's on.
 //
 // A block of 32 values with the largest magnitude m has the scale 2^max(floor(log2 m) - 2, -127); a value v becomes
@@ -165,27 +165,35 @@ __device__ __forceinline__ float max_abs(float a, float b, float c) {
 // is m's exponent field, so the scale's byte is max(field - 2, 0), and dividing by the scale is an exact product with a
 // power of two.  The bits of the largest magnitude say both the scale and, as infinities and NaN have the largest exponent
 // field, whether the block is a number at all (if not its scale is 255, whatever its codes).
-template <typename T>
-__device__ __forceinline__ uint32_t quantize8(const Eight<T>& x, int lane, uint32_t& scales) {
-    float v[8];
+template <typename T, int EIGHTS>
+__device__ __forceinline__ void quantize_lane(const Eight<T> (&x)[EIGHTS], int lane, uint32_t (&codes)[EIGHTS], uint32_t& scales) {
+    float v[EIGHTS][8], largest = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        uint32_t bits;
-        if constexpr (sizeof(T) == 2) bits = j & 1 ? x.w[j / 2] & 0xffff0000u : x.w[j / 2] << 16;
-        else bits = x.w[j];
-        v[j] = __uint_as_float(bits);
+    for (int i = 0; i < EIGHTS; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            uint32_t bits;
+            if constexpr (sizeof(T) == 2) bits = j & 1 ? x[i].w[j / 2] & 0xffff0000u : x[i].w[j / 2] << 16;
+            else bits = x[i].w[j];
+            v[i][j] = __uint_as_float(bits);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) largest = max_abs(largest, v[i][j], v[i][j + 1]);
     }
-    uint32_t most = __float_as_uint(max_abs(max_abs(v[0], v[1], v[2]), max_abs(v[3], v[4], v[5]), max_abs(v[6], v[7], v[7])));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    uint32_t most = __float_as_uint(largest);
+#pragma unroll
+    for (int o = 1; o < 4 / EIGHTS; o *= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     const uint32_t field = most >> 23;
     const uint32_t scale = field == 255 ? 255 : max(field, 2u) - 2;
     const float inverse = __uint_as_float((254 - min(scale, 253u)) << 23);           // 2^(127 - scale)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] *= inverse;
-    scales = scale << (2 * (lane & 12));
-    scales |= __shfl_xor_sync(0xffffffffu, scales, 4);
-    scales |= __shfl_xor_sync(0xffffffffu, scales, 8);
-    return pack8(v);
+    for (int i = 0; i < EIGHTS; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] *= inverse;
+        codes[i] = pack8(v[i]);
+    }
+    scales = scale << (8 * ((lane * EIGHTS >> 2) & 3));
+    scales |= __shfl_xor_sync(0xffffffffu, scales, 4 / EIGHTS);
+    scales |= __shfl_xor_sync(0xffffffffu, scales, 8 / EIGHTS);
 }
 }  // namespace mls_mx4

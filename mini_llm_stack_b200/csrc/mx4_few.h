@@ -66,24 +66,24 @@ __device__ __forceinline__ void quantise_slice(const FewProduct& p, int kb0, int
     int kb = worker / p.M, r = worker - kb * p.M;
     constexpr int AT_ONCE = 4;
     while (kb < n_kb) {
-        Eight<T> held[AT_ONCE];
+        Eight<T> held[AT_ONCE][1];
         int at_kb[AT_ONCE], at_r[AT_ONCE];
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
             at_kb[j] = kb, at_r[j] = r;
-            if (kb < n_kb) held[j] = load8<T, VEC>(x + r * p.ld, kb * BK, K);
+            if (kb < n_kb) held[j][0] = load8<T, VEC>(x + r * p.ld, kb * BK, K);
             kb += step_kb, r += step_r;
             if (r >= p.M) r -= p.M, ++kb;
         }
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
             if (at_kb[j] >= n_kb) break;
-            uint32_t scales;
-            const uint32_t codes = quantize8(held[j], lane, scales);
+            uint32_t scales, codes[1];
+            quantize_lane(held[j], lane, codes, scales);
             uint8_t* stage = rows + at_kb[j] * L::ROWS_STAGE;
             // (the 128-byte swizzle: a row's 16-byte pieces change places by the row's number)
             *reinterpret_cast<uint32_t*>(stage + at_r[j] * CODE_ROW + (((lane >> 2) ^ (at_r[j] & 7)) << 4) + (lane & 3) * 4) =
-                codes;
+                codes[0];
             if ((lane & 15) == 0)
                 *reinterpret_cast<uint32_t*>(stage + NR * CODE_ROW + (lane >> 4) * ATOM + row_in_atom(at_r[j])) = scales;
         }

@@ -1670,8 +1670,8 @@ class Ops:
             raise KernelError(f"{what}: at most {self.MX4_MOST_ROWS} slots")
         at, to = rows.data_ptr(), out.data_ptr()
         self._mx4_apart(at, ((shape[0] - 1) * ld + k) * (4 - 2 * code), to, slots * n * (4 - 2 * out_type), what)
-        # (many slots: every token is quantised once and copied to its slots; 12,288 slots of 2,048 tokens x 4,096 in 12 us
-        # where they took 27 one by one)
+        # (many slots: every token is quantised once and copied to its slots; 2,048 tokens x 4,096, six chosen, up: 127 us
+        # instead of 136, but 16 tokens 47 instead of 45)
         tokens = shape[0] if unit and top > 1 and slots * -(-k // 256) >= self.MX4_ONCE else 0
         codes, scales, t_codes, t_scales = self._mx4_scratch(slots, k, slots // 128 + n_experts + 1, tokens)
         self.launches += (2 if tokens else 1) - (-n_experts // 1024)
