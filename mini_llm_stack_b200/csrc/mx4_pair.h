@@ -272,12 +272,14 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
         // two runs of 32 columns a set: the first of 256 in the columns that the next accumulator may take
         constexpr int RUNS = L::NT / 32 / L::SETS, FREE_AT = L::NT == 256 ? RUNS / 2 - 1 : RUNS - 1;
         const bool vec = p.width % (p.out_type == MLS_BF16 ? 16 : 8) == 0 && reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
+        // (relaxed: the fence orders what was read from tensor memory; a release waits for the stores of the runs before as
+        // well, 22.5 us instead of 18.9 for 707 rows x 2,048 by 16,384 gated sums)
         auto arrive = [&](uint32_t bar) {
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
                 if (rank == 0) mbar_arrive(bar);
-                else mbar_arrive_remote(bar, 0);
+                else mbar_arrive_remote_relaxed(bar, 0);
             }
         };
         int it = 0;
