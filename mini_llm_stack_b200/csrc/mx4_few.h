@@ -166,6 +166,7 @@ __device__ __forceinline__ void few_block(const FewProduct& p, const CUtensorMap
     } else if (warp == 1) {
         // ---------------------------------------------------------------- instructions
         const uint32_t idesc0 = idesc_mx4(UMMA_M, NR, 0), idesc1 = idesc_mx4(UMMA_M, NR, 1);
+        chain_wait();                    // (the kernel before may take longer than a wait for the rows has)
         if (FUSED && !mbar_wait_warp(rows_full, 0)) timed_out = true;
         for (int g = 0; g < n_kb && !timed_out; ++g) {
             const int slot = g % stages;

@@ -46,6 +46,18 @@ def test_copies_land_before_the_block_ends(header):
     assert re.search(r"for \(int \w+ = [^;]*;[^)]*\)\s*if \(!mbar_wait\w*\([^;]*full[^;]*timed_out = true;", behind)
 
 
+@pytest.mark.parametrize("header", sorted(HEADERS))
+def test_bounded_waits_begin_behind_the_kernel_before(header):
+    """A wait's time does not run while the kernel in front, however long it takes, still does."""
+    common, *parts = re.split(r"\n    (?:if|\} else if|\} else) (?:\(warp == [01]\) )?\{\n", block(header))
+    if re.search(r"\n    chain_wait\(\);", block(header).split("// ----")[0].split("bool timed_out")[0]):
+        return
+    waiting = [p for p in parts if "mbar_wait" in p]
+    assert len(waiting) == 3
+    for part in waiting:
+        assert "chain_wait();" in part and part.index("chain_wait();") < part.index("mbar_wait")
+
+
 def test_every_wait_is_bounded():
     for p in CSRC.glob("mx4*"):
         text = re.sub(r"//[^\n]*", "", p.read_text())
