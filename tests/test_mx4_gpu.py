@@ -449,3 +449,65 @@ def test_refusals(ops):
             call()
     ops.linear_mx4(a, w, out)
     ops.check_status()
+
+
+# ------------------------------------------------------------------------------------- places beyond 32 bits
+def test_many_rows_are_quantised(ops):
+    """More than 2^32 values and 2^31 bytes of codes: repeated rows, whose codes repeat."""
+    k, once, times = 4096, 4096, 270
+    part = wide_rows(once, k, gen("many")).bfloat16().cuda()
+    x = part.expand(times, once, k).reshape(times * once, k)
+    assert x.numel() > 1 << 32
+    few, many = ops.quantize_mx4(part), ops.quantize_mx4(x)
+    assert many.codes.numel() > 1 << 31
+    assert bool((many.codes.view(times, -1) == few.codes.view(1, -1)).all())
+    assert bool((many.scales.view(times, -1) == few.scales.view(1, -1)).all())
+    want = torch.empty_like(part)
+    ops.mx4_values(few, want)
+    x.fill_(-5.0)
+    ops.mx4_values(many, x)
+    assert bool((x.view(times, once, k) == want).all())
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_large_outputs(ops, gated):
+    """An output of more than 2^32 values: rows from its start, its middle and its end."""
+    m, n, k = 70000, 62000, 64
+    g = gen("large", gated)
+    a = torch.randn(m, k, generator=g).bfloat16()
+    w = torch.randn(2, n, k, generator=g).bfloat16()
+    out = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    if gated:
+        ops.linear_glu_mx4(a.cuda(), ops.prepare_weight_mx4(w.cuda(), gate_up=True), out)
+    else:
+        ops.linear_mx4(a.cuda(), ops.prepare_weight_mx4(w[0].cuda()), out)
+    ops.check_status()
+    rows = torch.tensor([0, 1, 34999, 35000, 69887, 69888, 69998, 69999])
+    assert out.numel() > 1 << 32
+    qa, qw = plain.nearest(a[rows]), on_device(w.cuda()).cpu()
+    want, off = plain.product(qa, qw[0])
+    if gated:
+        up, off_up = plain.product(qa, qw[1])
+        want, off = plain.unit(want, up, off, off_up)
+    near(out[rows.cuda()].cpu(), want, off, torch.bfloat16)
+
+
+def test_large_outputs_by_expert(ops):
+    """Slots' rows of more than 2^32 values, and every token's choices twice the same expert."""
+    t, top, experts, d, f = 140000, 2, 3, 16384, 64
+    g = gen("large experts")
+    idx = torch.randint(0, experts, (t, 1), generator=g).expand(t, top).contiguous()
+    weight = torch.rand(t, top, generator=g) + 0.1
+    work = routed(idx, weight, experts)
+    y = torch.randn(t * top, f, generator=g).bfloat16()
+    w = torch.randn(experts, d, f, generator=g).bfloat16()
+    out = torch.empty(t * top, d, device="cuda")
+    assert out.numel() > 1 << 32
+    ops.expert_down_mx4(y.cuda(), ops.prepare_weight_mx4(w.cuda()), out, work, top, True)
+    ops.check_status()
+    order, flat, share = work["order"].cpu().long(), idx.reshape(-1), weight.reshape(-1).double()
+    qw = on_device(w.cuda()).cpu()
+    for p in (0, 1, 100000, 140000, 200000, t * top - 2, t * top - 1):
+        slot = int(order[p])
+        z, off = plain.product(plain.nearest(y[p:p + 1]), qw[flat[slot]])
+        near(out[slot:slot + 1].cpu(), z * share[slot], (off + z.abs() * plain.STEPS) * share[slot], torch.float32)
