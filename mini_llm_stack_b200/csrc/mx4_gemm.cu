@@ -34,9 +34,10 @@ mx4_product_kernel(const Product p, const __grid_constant__ CUtensorMap rows_map
 
 template <int NT, bool GROUPED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PairPlan<NT>::THREADS, 1)
-mx4_pair_kernel(const Product p, const __grid_constant__ CUtensorMap rows_map, const __grid_constant__ CUtensorMap w_map,
-                const __grid_constant__ CUtensorMap sf_rows_map, const __grid_constant__ CUtensorMap sf_w_map) {
-    pair_block<NT, GROUPED>(p, &rows_map, &w_map, &sf_rows_map, &sf_w_map);
+mx4_pair_kernel(const Product p, const __grid_constant__ CUtensorMap rows_map, const __grid_constant__ CUtensorMap half_map,
+                const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap sf_rows_map,
+                const __grid_constant__ CUtensorMap sf_w_map) {
+    pair_block<NT, GROUPED>(p, &rows_map, &half_map, &w_map, &sf_rows_map, &sf_w_map);
 }
 
 template <int NR, bool FUSED>
@@ -125,8 +126,9 @@ int launch_pair(const Product& p, const void* rows, const void* W, cudaStream_t 
     if (const int e = limit.set(mx4_pair_kernel<NT, GROUPED>, L::FIXED + 4 * (TABLE_EXPERTS + 1))) return e;
     const long long row_tiles = GROUPED ? p.M / TILE_ROWS + p.all_experts + 1 : (p.M + TILE_ROWS - 1) / TILE_ROWS;
     const long long w_tiles = (long long)p.n_experts * ((p.N + TILE_ROWS - 1) / TILE_ROWS);
-    CUtensorMap rows_map, w_map, sf_rows_map, sf_w_map;
-    if (!codes_map(rows, p.M, p.K, UMMA_M, &rows_map) || !codes_map(W, (long long)p.n_experts * p.N, p.K, NT / 2, &w_map) ||
+    CUtensorMap rows_map, half_map, w_map, sf_rows_map, sf_w_map;
+    if (!codes_map(rows, p.M, p.K, UMMA_M, &rows_map) || !codes_map(rows, p.M, p.K, UMMA_M / 2, &half_map) ||
+        !codes_map(W, (long long)p.n_experts * p.N, p.K, NT / 2, &w_map) ||
         !scales_map(p.sf_a, row_tiles, p.K, 1, &sf_rows_map) || !scales_map(p.sf_w, w_tiles, p.K, 2, &sf_w_map))
         return MLS_ERR_TENSOR_MAP;
     const long long tiles = GROUPED ? (long long)(p.M / L::ROWS) + (p.M < p.n_experts ? p.M : p.n_experts)
@@ -135,7 +137,7 @@ int launch_pair(const Product& p, const void* rows, const void* W, cudaStream_t 
     if (units > 0x3fffffffLL) return MLS_ERR_UNSUPPORTED;
     const int most = sm_count() / 2, pairs = (int)(units < most ? units : most);
     const int rc = launch_plain(mx4_pair_kernel<NT, GROUPED>, dim3(2 * pairs), dim3(L::THREADS),
-                                L::FIXED + (GROUPED ? 4 * (p.n_experts + 1) : 0), stream, p, rows_map, w_map, sf_rows_map, sf_w_map);
+                                L::FIXED + (GROUPED ? 4 * (p.n_experts + 1) : 0), stream, p, rows_map, half_map, w_map, sf_rows_map, sf_w_map);
     return rc ? rc : launch_status();
 }
 

@@ -89,6 +89,76 @@ __device__ __forceinline__ void store_run(OUT* out, const float (&v)[COUNT], int
     }
 }
 
+// 16 lanes of tensor memory x 32 columns: thread t gets, for i < 4, columns 8 i + 2 (t % 4) and the one behind it of lane t / 4 in
+// r[4 i], r[4 i + 1] and of lane t / 4 + 8 in r[4 i + 2], r[4 i + 3].
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t addr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+// Of four threads that hold columns 8 i + 2 t, 8 i + 2 t + 1 (i < 4; t: which of the four) in v[i], thread t gets columns 8 t to 8 t + 7:
+// a 4 x 4 transposition of pairs, by halves.
+__device__ __forceinline__ void gather_columns(uint32_t (&v)[4][2], int t) {
+#pragma unroll
+    for (int bit = 1; bit < 4; bit *= 2) {
+        const bool upper = t & bit;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i & bit) continue;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? v[i][x] : v[i | bit][x], bit);
+                (upper ? v[i][x] : v[i | bit][x]) = got;
+            }
+        }
+    }
+}
+
+// What a warp knows of the rows that it stores.  Whole lines (store_lines): thread t stores to the rows t / 4 + 8 z; else its lane's.
+struct To {
+    int row[4];
+    float share[4];
+    bool mine[4];
+};
+// The same runs for outputs of 32 bits that need no neighbours: a warp stores 128 bytes each to eight rows at a time (32 bytes
+// each to its 32 rows: 152 us instead of 146, at the same sizes).
+template <typename OUT, bool GROUPED, int RUNS, typename Read>
+__device__ __forceinline__ void store_lines(const Product& p, uint32_t d, int set, int sets, bool down, int columns, int n0,
+                                            bool any, const To& to, int lane, bool vec, Read read) {
+#pragma unroll 1
+    for (int i = 0; i < RUNS; ++i) {
+        const int c0 = ((down ? RUNS - 1 - i : i) * sets + set) * 32;
+        if (!any || c0 >= columns) {                 // (nothing to read)
+            read(i);
+            continue;
+        }
+        uint32_t x[2][16];
+        tmem_ld_16x32(d + c0, x[0]);
+        tmem_ld_16x32(d + (16u << 16) + c0, x[1]);
+        tmem_ld_wait();
+        read(i);
+        const int col = n0 + c0 + lane % 4 * 8;
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+            uint32_t w[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j][0] = x[z / 2][4 * j + z % 2 * 2], w[j][1] = x[z / 2][4 * j + z % 2 * 2 + 1];
+            gather_columns(w, lane % 4);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = __uint_as_float(w[j / 2][j % 2]);
+                if (GROUPED) v[j] *= to.share[z];
+                if (p.unit == RELU2) v[j] = fmaxf(v[j], 0.f) * fmaxf(v[j], 0.f);
+            }
+            if (to.mine[z]) store_run<OUT>((OUT*)p.out + (size_t)to.row[z] * p.width + col, v, p.width - col, vec);
+        }
+    }
+}
+
 // A warp's runs of 32 columns of the accumulator, for its 32 rows: this thread's goes to row `to`.  The set's runs lie `step`
 // columns apart, in the order in which they are to be read; `read(i)` is called behind the i-th one's reading.
 template <typename OUT, bool GROUPED, int RUNS, typename Read>
@@ -133,8 +203,8 @@ __device__ __forceinline__ void store_rows(const Product& p, uint32_t d, int set
 }
 
 template <int NT_, bool GROUPED>
-__device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* rows_map, const CUtensorMap* w_map,
-                                           const CUtensorMap* sf_rows_map, const CUtensorMap* sf_w_map) {
+__device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* rows_map, const CUtensorMap* half_map,
+                                           const CUtensorMap* w_map, const CUtensorMap* sf_rows_map, const CUtensorMap* sf_w_map) {
     using L = PairPlan<NT_>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_u32(smem_raw);
@@ -188,9 +258,15 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
             int g = 0;
             for (int i = first; i < units && !timed_out; i += step) {
                 const Unit u = unit_of<L::ROWS, GROUPED, L::NT>(p, i, w_tiles, start);
-                // (a second block without rows brings in none)
-                const bool second = u.rows > UMMA_M, with_rows = rank == 0 || second;
-                const uint32_t bytes = (second ? 2 : 1) * L::A_BYTES + 2 * (L::B_BYTES + 3 * SF_STAGE);
+                // (a second block without rows brings in none, one with up to 64 half a tile: what else lies in the stage ends in
+                // sums that nobody reads)
+                auto row_bytes = [&](int block) {
+                    const int rows = u.rows - block * UMMA_M;
+                    return rows <= 0 ? 0 : GROUPED && rows <= UMMA_M / 2 ? L::A_BYTES / 2 : L::A_BYTES;
+                };
+                const int mine = row_bytes((int)rank);
+                const CUtensorMap* from = mine == L::A_BYTES ? rows_map : half_map;
+                const uint32_t bytes = row_bytes(0) + row_bytes(1) + 2 * (L::B_BYTES + 3 * SF_STAGE);
                 const int row = u.row0 + (int)rank * UMMA_M, w_row = u.e * p.N + u.n0 + (int)rank * (columns(u) / 2);
                 const int sf_row = u.sf_tile + (int)rank, sf_w = u.e * sf_tiles + u.n0 / TILE_ROWS;
                 for (int kb = 0; kb < kblocks; ++kb, ++g) {
@@ -202,7 +278,7 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
                     const uint32_t a = base + slot * L::STAGE, bar = full(slot);
                     // both blocks' copies of the stage complete on the first one's barrier
                     if (rank == 0) mbar_arrive_expect_tx(bar, bytes);
-                    if (with_rows) tma_load_2d_pair(a, rows_map, kb * CODE_ROW, row, bar);
+                    if (mine) tma_load_2d_pair(a, from, kb * CODE_ROW, row, bar);
                     tma_load_2d_pair(a + L::A_BYTES, w_map, kb * CODE_ROW, w_row, bar);
                     tma_load_3d_pair(a + L::SF_A, sf_rows_map, 0, kb, sf_row, bar);
                     tma_load_3d_pair(a + L::SF_B, sf_w_map, 0, kb, sf_w, bar);
@@ -277,14 +353,47 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
         auto arrive = [&](uint32_t bar) {
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-                if (rank == 0) mbar_arrive(bar);
-                else mbar_arrive_remote_relaxed(bar, 0);
-            }
+            if (lane == 0) mbar_arrive_remote_relaxed(bar, 0);
         };
+        // Where this thread's rows go and the weights of their slots: numbers of slots read two units ahead, weights one, while
+        // instructions run and sums are stored (read when their unit's turn came: 146 us instead of 129 for 2,048 tokens down, six
+        // chosen of 64 experts of 4,096 x 1,408)
+        const bool lines = p.unit != GATED && p.out_type != MLS_BF16, look = GROUPED && (p.unit == DOWN || p.scale);
+        const int row = (int)rank * UMMA_M + q * 32;               // the warp's first
+        auto row_of = [&](int z) { return row + (lines ? lane / 4 + 8 * z : lane); };
+        auto unit_at = [&](int i) {
+            Unit u = {};                                           // (behind the last: no rows)
+            if (i < units) u = unit_of<L::ROWS, GROUPED, L::NT>(p, i, w_tiles, start);
+            return u;
+        };
+        struct Slots {
+            int at[4];
+        };
+        auto slots_of = [&](const Unit& u) {
+            Slots s;
+#pragma unroll
+            for (int z = 0; z < 4; ++z)
+                s.at[z] = look && (z == 0 || lines) && row_of(z) < u.rows ? p.order[u.row0 + row_of(z)] : 0;
+            return s;
+        };
+        struct Shares {
+            float at[4];
+        };
+        auto shares_of = [&](const Unit& u, const Slots& s) {
+            Shares f;
+#pragma unroll
+            for (int z = 0; z < 4; ++z)
+                f.at[z] = look && p.scale && (z == 0 || lines) && row_of(z) < u.rows ? p.weight[s.at[z]] : 1.f;
+            return f;
+        };
+        Unit u = unit_at(first), u1 = unit_at(first + step);
+        Slots slots = slots_of(u), slots1 = slots_of(u1);
+        Shares shares = shares_of(u, slots);
         int it = 0;
         for (int i = first; i < units; i += step, ++it) {
-            const Unit u = unit_of<L::ROWS, GROUPED, L::NT>(p, i, w_tiles, start);
+            const Unit u2 = unit_at(i + 2 * step);
+            const Slots slots2 = slots_of(u2);
+            const Shares shares1 = shares_of(u1, slots1);
             const int acc = it & 1;
             // (the columns in the middle first: an accumulator at the end begins there, one at the start ends there)
             const bool down = acc == 0;
@@ -293,15 +402,13 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
                 if (run == FREE_AT) arrive(acc_free(acc));
                 if (run == RUNS - 1) arrive(acc_empty(acc));
             };
-            // where this thread's row goes and the weight of its slot, read while the instructions still run
-            const int row = (int)rank * UMMA_M + q * 32;
-            const bool any = row < u.rows, mine = row + lane < u.rows;
-            int to = u.row0 + row + lane;
-            float share = 1.f;
-            if (GROUPED && mine && (p.unit == DOWN || p.scale)) {
-                const int s = p.order[to];
-                if (p.scale) share = p.weight[s];
-                if (p.unit == DOWN) to = s;
+            const bool any = row < u.rows;
+            To to;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                to.row[z] = GROUPED && p.unit == DOWN ? slots.at[z] : u.row0 + row_of(z);
+                to.share[z] = shares.at[z];
+                to.mine[z] = row_of(z) < u.rows;
             }
             if (!mbar_wait_warp(acc_full(acc), (it >> 1) & 1)) {
                 timed_out = true;
@@ -309,11 +416,15 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
             }
             tc_fence_after();
             const uint32_t at = d + ((uint32_t)(q * 32) << 16);
-            if (p.out_type == MLS_BF16)
-                store_rows<__nv_bfloat16, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, mine, to, share, vec,
-                                                         read);
+            if (lines)
+                store_lines<float, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, to, lane, vec, read);
+            else if (p.out_type == MLS_BF16)
+                store_rows<__nv_bfloat16, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, to.mine[0], to.row[0],
+                                                         to.share[0], vec, read);
             else
-                store_rows<float, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, mine, to, share, vec, read);
+                store_rows<float, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, to.mine[0], to.row[0],
+                                                 to.share[0], vec, read);
+            u = u1, u1 = u2, slots = slots1, slots1 = slots2, shares = shares1;
         }
     }
     if (timed_out && p.status) atomicOr(p.status, MLS_STATUS_TIMEOUT);
