@@ -143,14 +143,14 @@ int launch_pair(const Product& p, const void* rows, const void* W, cudaStream_t 
 
 // The ways of many rows, by the tile of a unit of work: 128 weights x 64 or 192 rows on one block, 256 rows x 192 or 256 weights on
 // a pair (routed: 256 x 256 only).  Units are dealt out in rounds of one a block or pair; a round takes so long for every
-// 256 of K, and so long for what its epilogue leaves visible (float32 sums of slots are 200 MB in a long prompt).  The
+// 256 of K, and so long for what its epilogue leaves visible (float32 sums of slots are 200 MB in a long prompt; pairs store them in whole lines).  The
 // cheapest way is taken.  Measured, us, in the order 64 / 192 / 192 on pairs / 256 on pairs, rows quantised already:
 //   256 rows x 14,336, 4,096 outputs       21.4 / 30.3 / 21.5 / 22.5     2,048 rows          125 / 82 / 54 / 42
 //   128 x 4,096, 28,672 gated              23.4 / 16.0 / 20.1 / 17.1     2,048 rows          266 / 134 / 102 / 95
 //   256 x 2,048, 2,048                     5.9 / 10.0 / 8.0 / 8.6        2,048 rows          15.6 / 15.7 / 11.6 / 9.3
 // and routed, the whole call, 64 / 192 / pairs (8b: 64 experts of 4,096 x 1,408, 6 chosen; 1b: 32 of 2,048 x 1,024, 4 chosen):
-//   8b, gate and up, 16 tokens  44.8 / 47.9 / 51.0, 600  98 / 88 / 92, 2,048  212 / 138 / 131
-//   1b, down, 600 tokens        29.4 / 36.1 / 34.5; 8b, 2,048 tokens  191 / 213 / 186
+//   8b, gate and up, 16 tokens  45 / 48 / 53, 600  94 / 84 / 90, 2,048  210 / 136 / 118
+//   1b, down, 200 tokens        18.0 / 19.5 / 20.9, 600  29.3 / 35.0 / 26.7; 8b, 2,048 tokens  188 / 201 / 127
 template <bool GROUPED>
 int launch(const Product& p, const void* rows, const void* W, cudaStream_t stream) {
     const double k = (p.K + BK - 1) / BK, gated = p.unit == GATED ? 1 : 0, slots = GROUPED && p.unit == DOWN ? 1 : 0;
@@ -168,7 +168,7 @@ int launch(const Product& p, const void* rows, const void* W, cudaStream_t strea
     const double t[4] = {cost(64, 128, blocks, 0.335, 0.45, 0), cost(192, 128, blocks, of_192 > 0.345 ? of_192 : 0.345,
                                                                      0.9 + 2.5 * slots, 0),
                          GROUPED ? 1e30 : cost(256, 192, pairs, 0.355, 0.5 + 0.8 * gated, 1),
-                         GROUPED ? cost(256, 256, pairs, 0.30 + 0.0004 * rows_in(256), 0.9 + 0.6 * gated + 2 * slots, 2)
+                         GROUPED ? cost(256, 256, pairs, 0.30 + 0.0003 * rows_in(256), 0.6 + 0.6 * gated, 1)
                                  : cost(256, 256, pairs, 0.365, 0.9 + 0.6 * gated, 1)};
     int best = 0;
     for (int way = 1; way < 4; ++way)
