@@ -7,10 +7,9 @@
 // both halves.  Each block holds the scales of its own rows and of all the tile's weights.
 //
 // The batch's rows lie on the 128-row side: a thread of the epilogue then holds neighbouring outputs of one row, gate and up of
-// the same output among them, and stores whole sectors of 32 bytes.  (With the weights there, a warp's stores are 64 or 128
-// bytes of a row each: 2,048 rows x 28,672 x 4,096 with SwiGLU took 213 us, of which the epilogue was 110; 2,048 tokens through 64
-// experts of 4,096 x 1,408, six chosen, 135 us down instead of 116.  Up it is no matter, 121 and 119: what tiles of 256 rows waste
-// on experts of few the wider stores win back.)
+// the same output among them, and stores whole sectors of 32 bytes, or with a transposition between four threads lines of 128.
+// (With the weights there, a warp's stores are 64 or 128 bytes of a row each: 2,048 rows x 28,672 x 4,096 with SwiGLU took 213 us
+// instead of 95, 110 of them the epilogue.)
 //
 // Tensor memory: ACC_COLS columns of accumulators, every second one from the first column on, the others up to the last, so that
 // two that fit beside one another overlap: the epilogue of one lies under the instructions of the next.  NT = 192 always fits;
@@ -19,7 +18,12 @@
 //
 // Hand-overs inside the pair, as in the bfloat16 product: full[s] (first block) counts both blocks' copies; empty[s] and acc_full[a]
 // arrive on both blocks' barriers; acc_free[a] and acc_empty[a] (first block) take the arrivals of both blocks' epilogue warps,
-// when they have read the half of an accumulator that the next may take, and all of it.  No load is multicast.  These kernels are launched plainly: chained behind a long quantisation of rows a run under a profiler did not end.
+// when they have read the half of an accumulator that the next may take, and all of it.  No load is multicast.  These kernels are launched
+// plainly: chained behind a long quantisation of rows a run under a profiler did not end.
+//
+// What bounds it: operands out of L2 (2,048 x 14,336 by 4,096 in 44 us, 5.5 PFLOP/s; 2,048 tokens, six of 64 experts, gate and up
+// 2 x 1,408 of 4,096 in 100 us, 70 without copies), and where float32 sums of slots are stored, memory (down 1,408 by 4,096 in 84 us
+// for 450 MB).
 #pragma once
 #include "mx4_gemm.h"
 
