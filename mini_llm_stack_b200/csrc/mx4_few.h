@@ -14,6 +14,11 @@ constexpr int FEW_STAGES = 4;
 constexpr int FEW_WORKERS = 8;                        // warps that quantise, read the sums and store them
 constexpr int FEW_THREADS = 32 * (2 + FEW_WORKERS);
 constexpr int FEW_SLICES = 8;                         // blocks of a cluster, at most
+// The least shared memory of a block: four of them fill an SM, so that the 128 columns of tensor memory that each holds are always
+// there.  Blocks of a cluster hold them while they wait for one another; with more blocks than columns two clusters
+// could each wait for what the other has.  Nor do they fit beside a pair of blocks of this or the bfloat16 product, which wait for
+// each other in the same way and hold every column.
+constexpr int FEW_LEAST = 48 * 1024;
 constexpr int FEW_SLICE = 12;                         // stages of K of a slice, at most (FUSED: two blocks an SM)
 
 struct FewProduct {
@@ -38,6 +43,7 @@ struct FewPlan {
     static constexpr int SF_COLS_STAGE = 2 * SF_COLS;
     static constexpr int SF_AT = NR;
     static constexpr int COLS = pow2_at_least(SF_AT + FEW_STAGES * SF_COLS_STAGE);
+    static_assert(COLS * (227 * 1024 / FEW_LEAST) <= 512, "tensor memory of the blocks that fit an SM");
     // a slice's stages (as many as it has, up to FEW_STAGES), FUSED its rows' codes and scales, barriers.  The sums
     // [NR][128] take the place of the stages, once the instructions are done.
     __host__ __device__ static constexpr int stages(int slice) { return slice < FEW_STAGES ? slice : FEW_STAGES; }
@@ -46,7 +52,10 @@ struct FewPlan {
         const int loads = rows(slice) + (FUSED ? slice * ROWS_STAGE : 0), sums = NR * UMMA_M * 4;
         return loads > sums ? loads : sums;
     }
-    __host__ __device__ static constexpr int total(int slice) { return bars(slice) + 8 * (2 * FEW_STAGES + 2) + 16 + 1024; }
+    __host__ __device__ static constexpr int total(int slice) {
+        const int bytes = bars(slice) + 8 * (2 * FEW_STAGES + 2) + 16 + 1024;
+        return bytes > FEW_LEAST ? bytes : FEW_LEAST;
+    }
 };
 
 __device__ __forceinline__ float load_cluster_f32(uint32_t addr, uint32_t cta) {

@@ -122,6 +122,7 @@ int launch_nt(const Product& p, const void* rows, const void* W, cudaStream_t st
 template <int NT, bool GROUPED>
 int launch_pair(const Product& p, const void* rows, const void* W, cudaStream_t stream) {
     using L = PairPlan<NT>;
+    static_assert(L::FIXED + FEW_LEAST > 227 * 1024, "no block of a product of few rows beside a pair's");
     static SharedLimit limit;
     if (const int e = limit.set(mx4_pair_kernel<NT, GROUPED>, L::FIXED + 4 * (TABLE_EXPERTS + 1))) return e;
     const long long row_tiles = GROUPED ? p.M / TILE_ROWS + p.all_experts + 1 : (p.M + TILE_ROWS - 1) / TILE_ROWS;
