@@ -511,3 +511,46 @@ def test_large_outputs_by_expert(ops):
         slot = int(order[p])
         z, off = plain.product(plain.nearest(y[p:p + 1]), qw[flat[slot]])
         near(out[slot:slot + 1].cpu(), z * share[slot], (off + z.abs() * plain.STEPS) * share[slot], torch.float32)
+
+
+def test_two_models_at_once(ops):
+    """Calls of two runtimes on two streams, few rows, many rows and routed ones side by side."""
+    g = gen("two")
+    other = Runtime("cuda:0", torch.bfloat16).ops
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    jobs = []
+    for own in (ops, other):
+        w = own.prepare_weight_mx4((torch.randn(3000, 2100, generator=g) * 0.1).bfloat16().cuda())
+        pair = own.prepare_weight_mx4((torch.randn(2, 2100, 3000, generator=g) * 0.1).bfloat16().cuda(), gate_up=True)
+        calls = []
+        for m in (1, 9, 40, 300, 1100):
+            a = torch.randn(m, 2100, generator=g).bfloat16().cuda()
+            calls.append((own, w, pair, a, torch.empty(m, 3000, dtype=torch.bfloat16, device="cuda"),
+                          torch.empty(m, 2100, device="cuda")))
+        jobs.append(calls)
+
+    def run(call):
+        own, w, pair, a, mid, out = call
+        own.linear_mx4(a, w, mid)
+        own.linear_glu_mx4(mid, pair, out)
+
+    want = []
+    for calls in jobs:
+        for call in calls:
+            run(call)
+        want.append([call[5].clone() for call in calls])
+    torch.cuda.synchronize()
+    for call in sum(jobs, []):
+        call[5].fill_(-1.0)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i in range(len(jobs[0])):
+            for calls, stream in zip(jobs, streams):
+                with torch.cuda.stream(stream):
+                    run(calls[i])
+    torch.cuda.synchronize()
+    for calls, results in zip(jobs, want):
+        for call, result in zip(calls, results):
+            assert torch.equal(call[5], result)
+    ops.check_status()
+    other.check_status()
