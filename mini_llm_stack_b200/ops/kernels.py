@@ -172,6 +172,14 @@ class Mx4:
             self._slice = -(-steps // slices) if slices else 0
         return self._slice
 
+    def __deepcopy__(self, memo):
+        twin = Mx4(self.shape, self.device, self.gate_up)      # (addresses are its own memory's)
+        twin.data.copy_(self.data)
+        return twin
+
+    def __reduce__(self):
+        raise TypeError("Mx4 is an address on a device: keep the matrix that it was made of, or its codes and scales")
+
     @property
     def codes(self):
         return self.data[self.data.numel() - self.rows * self.pitch(self.k):].view(self.rows, self.pitch(self.k))

@@ -1,5 +1,8 @@
 """4-bit microscaled rows: sizes in memory, what is refused before anything reaches a device, the engine's option."""
 
+import copy
+import pickle
+
 import pytest
 import torch
 
@@ -115,3 +118,16 @@ def test_the_engines_option():
     with pytest.raises(ConfigError, match="ffn_weights"):
         EngineOptions(ffn_weights="int4")
     EngineOptions(device="cpu").check_against("bfloat16", "cpu", "mxfp4")     # asks for nothing
+
+
+def test_copies_have_their_own_memory():
+    q = Mx4((2, 3, 40), "cpu", gate_up=False)
+    q.data.copy_(torch.arange(q.data.numel()) % 251)
+    q.settled = True
+    twin = copy.deepcopy({"w": q})["w"]
+    assert torch.equal(twin.data, q.data) and twin.shape == q.shape and twin.data.data_ptr() != q.data.data_ptr()
+    assert twin.scales_at == twin.data.data_ptr() and twin.codes_at - twin.scales_at == q.codes_at - q.scales_at
+    assert not twin.settled
+    for refused in (copy.copy, pickle.dumps):
+        with pytest.raises(TypeError):
+            refused(q)
