@@ -81,27 +81,56 @@ mx4_quantize_kernel(const T* __restrict__ x, long long ld, const Tasks tasks, in
     }
 }
 
-// The sorted slot p of a routed step gets the codes and scales of its token: a warp a slot, 16 bytes of codes and four of scales a
-// lane at a time.
+// Where the slots of a routed step lie among its sorted rows: the row of codes, and that of scales counted in tiles of 128.
 __global__ void __launch_bounds__(256)
-mx4_spread_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int slots, int K, const RowMap map,
-                  uint8_t* __restrict__ to_codes, uint8_t* __restrict__ to_scales) {
+mx4_places_kernel(const RowMap map, int slots, int2* __restrict__ places) {
     chain_release();
     chain_wait();
-    const int p = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int p = blockIdx.x * blockDim.x + threadIdx.x;
     if (p >= slots) return;
     const int slot = map.order[p], e = map.idx[slot];
-    if (e >= map.n_experts) return;                  // a slot of an output without weights: nobody reads it
-    const int token = slot / map.top, o = map.offsets[e], pieces = pitch_of(K) / 16, atoms = atoms_of(K);
-    const uint4* from = reinterpret_cast<const uint4*>(codes) + (size_t)token * pieces;
-    uint4* to = reinterpret_cast<uint4*>(to_codes) + (size_t)p * pieces;
-#pragma unroll 4
-    for (int i = lane; i < pieces; i += 32) to[i] = from[i];
-    const uint8_t* sf = scales + (size_t)(token / TILE_ROWS) * atoms * ATOM + row_in_atom(token % TILE_ROWS);
-    uint8_t* to_sf = to_scales + (size_t)(first_tile(o, e) + (p - o) / TILE_ROWS) * atoms * ATOM +
-                     row_in_atom((p - o) % TILE_ROWS);
-    for (int i = lane; i < atoms; i += 32)
-        *reinterpret_cast<uint32_t*>(to_sf + (size_t)i * ATOM) = *reinterpret_cast<const uint32_t*>(sf + (size_t)i * ATOM);
+    int2 place = {-1, 0};                            // (a slot of an output without weights: nobody reads it)
+    if (e < map.n_experts) {
+        const int o = map.offsets[e];
+        place = {p, first_tile(o, e) * TILE_ROWS + p - o};
+    }
+    places[slot] = place;
+}
+
+// A token is quantised once and stored to all of its slots: a warp's task is 512 values of a token.  What bounds it is what L2 takes
+// in, 27 MB for 12,288 slots of 4,096, the scales among them in words of four bytes: 11.5 us and 2.9 for the places (the tokens'
+// codes and scales as rows of their own, copied to the slots by a second kernel: 17).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256)
+mx4_tokens_kernel(const T* __restrict__ x, long long ld, const Tasks tasks, int K, int top, int slots, int tiles,
+                  const int2* __restrict__ places, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    chain_release();
+    chain_wait();
+    const int pitch = pitch_of(K), atoms = atoms_of(K), lane = threadIdx.x & 31;
+    const unsigned first = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    unsigned token = first / tasks.chunks, chunk = first - token * tasks.chunks;
+    for (; token < tasks.rows; tasks.next(token, chunk)) {
+        const int k0 = (int)chunk * QUANTIZE_PART + lane * 16;
+        const T* row = x + (long long)token * ld;
+        const Eight<T> held[2] = {load8<T, VEC>(row, k0, K), load8<T, VEC>(row, k0 + 8, K)};
+        const int byte = (int)chunk * (QUANTIZE_PART / 2) + lane * 8, atom = (int)chunk * 4 + (lane >> 3);
+        uint32_t word = 0, packed[2];
+        for (int j0 = 0; j0 < top; j0 += 32) {
+            const int2 mine = j0 + lane < top ? places[(size_t)token * top + j0 + lane] : make_int2(-1, 0);
+            if (j0 == 0) quantize_lane(held, lane, packed, word);
+            const int n = min(32, top - j0);
+            for (int j = 0; j < n; ++j) {
+                const int to = __shfl_sync(0xffffffffu, mine.x, j), at = __shfl_sync(0xffffffffu, mine.y, j);
+                // (a place that the routing's arrays left out is none)
+                if ((unsigned)to >= (unsigned)slots || (unsigned)at >= (unsigned)tiles * TILE_ROWS) continue;
+                if (byte < pitch)
+                    *reinterpret_cast<uint2*>(codes + (size_t)to * pitch + byte) = make_uint2(packed[0], packed[1]);
+                if ((lane & 7) == 0 && atom < atoms)
+                    *reinterpret_cast<uint32_t*>(scales + ((size_t)(at / TILE_ROWS) * atoms + atom) * ATOM +
+                                                 row_in_atom(at % TILE_ROWS)) = word;
+            }
+        }
+    }
 }
 
 // What codes and scales stand for, in the same tasks.  A lane takes PER neighbouring values, 16 bytes of output, once in 256
@@ -197,6 +226,18 @@ int quantize(const void* x, long long ld, long long rows, int K, const RowMap& m
                            : launch_plain(kernel, dim3(blocks), dim3(256), 0, stream, (const T*)x, ld, tasks, K, map, codes, scales);
     return rc ? rc : launch_status();
 }
+
+template <typename T>
+int tokens_to_slots(const void* x, long long ld, long long tokens, int K, const RowMap& map, long long slots, const int2* places,
+                    uint8_t* codes, uint8_t* scales, cudaStream_t stream) {
+    Tasks tasks;
+    unsigned blocks;
+    if (!tasks_of(tokens, K, QUANTIZE_PART, 1, tasks, blocks)) return MLS_ERR_UNSUPPORTED;
+    auto* kernel = aligned16(x) && ld % (16 / (int)sizeof(T)) == 0 ? mx4_tokens_kernel<T, true> : mx4_tokens_kernel<T, false>;
+    const int rc = launch_plain(kernel, dim3(blocks), dim3(256), 0, stream, (const T*)x, ld, tasks, K, map.top, (int)slots,
+                                (int)(slots / TILE_ROWS + map.n_experts + 1), places, codes, scales);
+    return rc ? rc : launch_status();
+}
 }  // namespace
 
 namespace mls_mx4 {
@@ -205,11 +246,14 @@ int quantize_rows(const void* x, int dtype, long long ld, long long rows, int K,
     return dtype == MLS_BF16 ? quantize<__nv_bfloat16>(x, ld, rows, K, map, codes, scales, chained, stream)
                              : quantize<float>(x, ld, rows, K, map, codes, scales, chained, stream);
 }
-int spread_rows(const uint8_t* codes, const uint8_t* scales, long long slots, int K, const RowMap& map, uint8_t* to_codes,
-                uint8_t* to_scales, cudaStream_t stream) {
-    const int rc = launch_plain(mx4_spread_kernel, dim3((unsigned)((slots + 7) / 8)), dim3(256), 0, stream, codes, scales,
-                                (int)slots, K, map, to_codes, to_scales);
-    return rc ? rc : launch_status();
+int quantize_tokens(const void* x, int dtype, long long ld, long long tokens, int K, const RowMap& map, long long slots,
+                    void* places, uint8_t* codes, uint8_t* scales, cudaStream_t stream) {
+    const int rc = launch_plain(mx4_places_kernel, dim3((unsigned)((slots + 255) / 256)), dim3(256), 0, stream, map, (int)slots,
+                                (int2*)places);
+    if (rc) return rc;
+    return dtype == MLS_BF16
+               ? tokens_to_slots<__nv_bfloat16>(x, ld, tokens, K, map, slots, (const int2*)places, codes, scales, stream)
+               : tokens_to_slots<float>(x, ld, tokens, K, map, slots, (const int2*)places, codes, scales, stream);
 }
 }  // namespace mls_mx4
 

@@ -94,9 +94,9 @@ static inline int launch_plain(void (*kernel)(Params...), dim3 grid, dim3 block,
 // Rows [rows, K] of float32 or bfloat16, ld values apart, into codes and scales.
 int quantize_rows(const void* x, int dtype, long long ld, long long rows, int K, const RowMap& map, uint8_t* codes,
                   uint8_t* scales, bool chained, cudaStream_t stream);
-// Rows that are codes and scales already, gathered into the sorted slots of a routed step (map.gather).
-int spread_rows(const uint8_t* codes, const uint8_t* scales, long long slots, int K, const RowMap& map, uint8_t* to_codes,
-                uint8_t* to_scales, cudaStream_t stream);
+// The tokens' rows [tokens, K] once each, into all of their sorted slots; places: 8 bytes a slot of scratch.
+int quantize_tokens(const void* x, int dtype, long long ld, long long tokens, int K, const RowMap& map, long long slots,
+                    void* places, uint8_t* codes, uint8_t* scales, cudaStream_t stream);
 
 // Eight neighbouring values of a row as they lie (zeros behind the row's end); VEC: at a 16-byte place.
 template <typename T>

@@ -232,10 +232,10 @@ static int product(int unit, const void* rows, int rows_type, long long ld, void
 }
 
 // Expert by expert: the slots of a routed step and w [E, 1 or 2, N, K].  The rows (sorted, or gathered from the tokens')
-// are quantised into a and sf_a first: `tokens` rows once each into t and sf_t and from there into their slots, or (tokens == 0)
-// every slot's by itself.
-static int expert_product(int unit, const void* rows, int rows_type, long long ld, int top, int gather, int tokens, void* t,
-                          void* sf_t, void* a, void* sf_a, const void* w, const void* sf_w, void* out, int out_type,
+// are quantised into a and sf_a first, every slot's by itself, or with `places` (8 bytes a slot of scratch; gather only) every
+// token's once for all of its slots.
+static int expert_product(int unit, const void* rows, int rows_type, long long ld, int top, int gather, void* places, void* a,
+                          void* sf_a, const void* w, const void* sf_w, void* out, int out_type,
                           int n_slots, int n_experts, int N, int K, const int* order, const int* idx, const int* offsets,
                           const float* weight, int scale, float alpha, float limit, int* status, void* stream_) {
     if (n_slots <= 0 || N <= 0 || n_experts <= 0) return 0;
@@ -243,10 +243,8 @@ static int expert_product(int unit, const void* rows, int rows_type, long long l
     const cudaStream_t stream = (cudaStream_t)stream_;
     const RowMap map{n_slots, 0, order, idx, offsets, top, n_experts, gather};
     int rc;
-    if (tokens > 0) {
-        rc = quantize_rows(rows, rows_type, ld, tokens, K, RowMap{tokens, 0, nullptr, nullptr, nullptr, 1, 0, 0}, (uint8_t*)t,
-                           (uint8_t*)sf_t, false, stream);
-        if (!rc) rc = spread_rows((const uint8_t*)t, (const uint8_t*)sf_t, n_slots, K, map, (uint8_t*)a, (uint8_t*)sf_a, stream);
+    if (places) {
+        rc = quantize_tokens(rows, rows_type, ld, n_slots / top, K, map, n_slots, places, (uint8_t*)a, (uint8_t*)sf_a, stream);
     } else {
         rc = quantize_rows(rows, rows_type, ld, n_slots, K, map, (uint8_t*)a, (uint8_t*)sf_a, chained(n_slots, K), stream);
     }
@@ -272,13 +270,13 @@ MLS_API int mls_mx4_product(int unit, const void* rows, int rows_type, long long
                        status, stream);
     });
 }
-MLS_API int mls_mx4_expert_product(int unit, const void* rows, int rows_type, long long ld, int top, int gather, int tokens,
-                                   void* t, void* sf_t, void* a, void* sf_a, const void* w, const void* sf_w, void* out,
+MLS_API int mls_mx4_expert_product(int unit, const void* rows, int rows_type, long long ld, int top, int gather, void* places,
+                                   void* a, void* sf_a, const void* w, const void* sf_w, void* out,
                                    int out_type, int n_slots, int n_experts, int N, int K, const int* order, const int* idx,
                                    const int* offsets, const float* weight, int scale, float alpha, float limit, int* status,
                                    void* stream) {
     return guarded([&] {
-        return expert_product(unit, rows, rows_type, ld, top, gather, tokens, t, sf_t, a, sf_a, w, sf_w, out, out_type, n_slots,
+        return expert_product(unit, rows, rows_type, ld, top, gather, places, a, sf_a, w, sf_w, out, out_type, n_slots,
                               n_experts, N, K, order, idx, offsets, weight, scale, alpha, limit, status, stream);
     });
 }

@@ -1008,7 +1008,7 @@ class Ops:
                                     [_I, _P, _I, _LL, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _F,
                                      _P, _P]),
                    "expert_product": _decl(lib, "mls_mx4_expert_product",
-                                           [_I, _P, _I, _LL, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I,
+                                           [_I, _P, _I, _LL, _I, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I,
                                             _P, _P, _P, _P, _I, _F, _F, _P, _P])}
         elif name == "shortconv":
             fns = {"qk": _decl(lib, "mls_qk_conv_norm_rope_store",
@@ -1479,7 +1479,7 @@ class Ops:
     # ------------------------------------------------- 4-bit microscaled rows and weights
     MX4_MOST_K = 1 << 20     # values of a row
     MX4_MOST_ROWS = 1 << 28  # rows of a matrix, and of a weight's matrices together
-    MX4_ONCE = 1 << 16       # slots x steps of 256 of K from which on tokens are quantised once
+    MX4_ONCE = 1 << 15       # slots x steps of 256 of K from which on tokens are quantised once
     MX4_FUSED_TASKS = 64     # 256 values of a row each: with so many a block the product quantises its rows itself
 
     def _mx4(self, name: str):
@@ -1582,20 +1582,16 @@ class Ops:
             held.settled = True
         return held
 
-    def _mx4_scratch(self, m: int, k: int, tiles: int, tokens: int = 0) -> tuple:
-        """Addresses of the codes and scales of a product's rows in scratch memory, and of those of the tokens that they are
-        gathered from."""
-        pitch, tile = Mx4.pitch(k), Mx4.tile_bytes(k)
-        token_tiles = (tokens + 127) // 128
-        held = self.scratch("mx4_rows", ((m + tokens) * pitch + (tiles + token_tiles) * tile) // 4)
+    def _mx4_scratch(self, m: int, k: int, tiles: int, more: int = 0) -> tuple:
+        """Addresses of the codes and scales of a product's rows in scratch memory, and of `more` bytes behind them."""
+        sf_bytes, bytes_ = tiles * Mx4.tile_bytes(k), m * Mx4.pitch(k)
+        held = self.scratch("mx4_rows", (sf_bytes + bytes_ + more) // 4)
         if torch.cuda.is_current_stream_capturing() and held is not self._mx4_captured:
             # a graph goes on writing there: the memory stays, whatever later products need
             self._mx4_captured = held
             self._mx4_kept.append(held)
         sf = held.data_ptr()
-        sf_tokens = sf + tiles * tile
-        codes = sf_tokens + token_tiles * tile
-        return codes, sf, codes + m * pitch, sf_tokens
+        return sf + sf_bytes, sf, sf + sf_bytes + bytes_
 
     def _product_mx4(self, unit: int, a, w: Mx4, out, what: str, alpha=1.0, limit=0.0) -> None:
         if w.__class__ is not Mx4 or w.lead or w.gate_up != (unit == 1):
@@ -1629,7 +1625,7 @@ class Ops:
             self._mx4_apart(rows, ((m - 1) * ld + k) * (4 - 2 * code), to, m * n * (4 - 2 * out_type), what)
             fused = 0 < few <= 12 and m <= 16 and m * few <= self.MX4_FUSED_TASKS
             if not fused:
-                codes, scales, _, _ = self._mx4_scratch(m, k, (m + 127) // 128)
+                codes, scales, _ = self._mx4_scratch(m, k, (m + 127) // 128)
                 self.launches += 1
         self.launches += 1
         rc = self._mx4("product")(unit, rows, code, ld, codes, scales, w.codes_at, w.scales_at, to, out_type, m, n, k, few, fused,
@@ -1678,13 +1674,13 @@ class Ops:
             raise KernelError(f"{what}: at most {self.MX4_MOST_ROWS} slots")
         at, to = rows.data_ptr(), out.data_ptr()
         self._mx4_apart(at, ((shape[0] - 1) * ld + k) * (4 - 2 * code), to, slots * n * (4 - 2 * out_type), what)
-        # (many slots: every token is quantised once and copied to its slots; 2,048 tokens x 4,096, six chosen, up: 127 us
-        # instead of 136, but 16 tokens 47 instead of 45)
-        tokens = shape[0] if unit and top > 1 and slots * -(-k // 256) >= self.MX4_ONCE else 0
-        codes, scales, t_codes, t_scales = self._mx4_scratch(slots, k, slots // 128 + n_experts + 1, tokens)
-        self.launches += (2 if tokens else 1) - (-n_experts // 1024)
+        # (many slots: every token is quantised once for all of them; 2,048 tokens x 4,096, six chosen, up: 118 us instead of 129,
+        # 400 77 instead of 78.5, but 16 tokens 47 instead of 45)
+        once = unit != 0 and top > 1 and slots * -(-k // 256) >= self.MX4_ONCE
+        codes, scales, places = self._mx4_scratch(slots, k, slots // 128 + n_experts + 1, 8 * slots if once else 0)
+        self.launches += (2 if once else 1) - (-n_experts // 1024)
         rc = self._mx4("expert_product")(
-            unit, at, code, ld, top, unit != 0, tokens, t_codes, t_scales, codes, scales, w.codes_at, w.scales_at, to, out_type,
+            unit, at, code, ld, top, unit != 0, places if once else None, codes, scales, w.codes_at, w.scales_at, to, out_type,
             slots, n_experts, n, k, order.data_ptr(), idx.data_ptr(), offsets.data_ptr(), weight.data_ptr(), scale, alpha,
             limit, self._status_at, self._stream())
         if rc:

@@ -554,3 +554,10 @@ def test_two_models_at_once(ops):
             assert torch.equal(call[5], result)
     ops.check_status()
     other.check_status()
+
+
+@pytest.mark.parametrize("kind", ["silu", "relu2"])
+def test_more_choices_than_lanes(ops, kind):
+    """Tokens that are quantised once for 36 slots each."""
+    assert 600 * 36 * 2 >= ops.MX4_ONCE
+    test_products_by_expert(ops, 600, 40, 2, 36, 300, 48, "even", kind)
