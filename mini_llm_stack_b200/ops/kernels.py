@@ -1479,6 +1479,7 @@ class Ops:
     # ------------------------------------------------- 4-bit microscaled rows and weights
     MX4_MOST_K = 1 << 20     # values of a row
     MX4_MOST_ROWS = 1 << 28  # rows of a matrix, and of a weight's matrices together
+    MX4_MOST_EXPERTS = 1 << 16
     MX4_ONCE = 1 << 15       # slots x steps of 256 of K from which on tokens are quantised once
     MX4_FUSED_TASKS = 64     # 256 values of a row each: with so many a block the product quantises its rows itself
 
@@ -1672,6 +1673,8 @@ class Ops:
             return
         if slots > self.MX4_MOST_ROWS:
             raise KernelError(f"{what}: at most {self.MX4_MOST_ROWS} slots")
+        if n_experts > self.MX4_MOST_EXPERTS:
+            raise KernelError(f"{what}: at most {self.MX4_MOST_EXPERTS} experts")
         at, to = rows.data_ptr(), out.data_ptr()
         self._mx4_apart(at, ((shape[0] - 1) * ld + k) * (4 - 2 * code), to, slots * n * (4 - 2 * out_type), what)
         # (many slots: every token is quantised once for all of them; 2,048 tokens x 4,096, six chosen, up: 118 us instead of 129,

@@ -131,3 +131,11 @@ def test_copies_have_their_own_memory():
     for refused in (copy.copy, pickle.dumps):
         with pytest.raises(TypeError):
             refused(q)
+
+
+def test_more_experts_than_places_are_numbered_for(ops):
+    many = Mx4((70000, 1, 1), "cpu")
+    work = {"order": torch.zeros(2, dtype=torch.int32), "idx": torch.zeros(2, dtype=torch.int32),
+            "offsets": torch.zeros(70001, dtype=torch.int32), "weight": torch.zeros(2)}
+    with pytest.raises(KernelError, match="experts"):
+        ops.expert_relu_squared_mx4(torch.zeros(1, 1), many, torch.zeros(2, 1), work, 2, False)
