@@ -231,7 +231,7 @@ class Ops:
         self._sample = _decl(core, "mls_sample", [_P, _P, _P, _P, _I, _I, _P, _P])
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._status_at = self.status.data_ptr()
-        self._mx4_captured, self._mx4_kept = None, []
+        self._mx4_rows: dict = {}                # quantised rows of the 4-bit products, by stream
         self._attention_libs: dict = {}
         self._attention_lib_handles: dict = {}
         self._split_ctas_per_sm: dict = {}       # head size -> CTAs of the split kernel an SM holds
@@ -1583,16 +1583,22 @@ class Ops:
             held.settled = True
         return held
 
-    def _mx4_scratch(self, m: int, k: int, tiles: int, more: int = 0) -> tuple:
-        """Addresses of the codes and scales of a product's rows in scratch memory, and of `more` bytes behind them."""
-        sf_bytes, bytes_ = tiles * Mx4.tile_bytes(k), m * Mx4.pitch(k)
-        held = self.scratch("mx4_rows", (sf_bytes + bytes_ + more) // 4)
-        if torch.cuda.is_current_stream_capturing() and held is not self._mx4_captured:
-            # a graph goes on writing there: the memory stays, whatever later products need
-            self._mx4_captured = held
-            self._mx4_kept.append(held)
+    def _mx4_scratch(self, stream: int, m: int, k: int, tiles: int, more: int = 0) -> tuple:
+        """Addresses of the codes and scales of a product's rows in scratch memory, and of `more` bytes behind them.  Every
+        stream has its own, and calls of a captured graph take the graph's: neither other streams' calls nor other graphs
+        write there."""
+        sf_bytes, row_bytes = tiles * Mx4.tile_bytes(k), m * Mx4.pitch(k)
+        size = sf_bytes + row_bytes + more
+        if torch.cuda.is_current_stream_capturing():
+            # (its next allocation may have the same memory: that call's kernels follow this one's)
+            held = torch.empty(size, dtype=torch.uint8, device=self.device)
+        else:
+            held = self._mx4_rows.get(stream)
+            if held is None or held.numel() < size:
+                held = torch.empty(max(size, 1 << 18), dtype=torch.uint8, device=self.device)
+                self._mx4_rows[stream] = held
         sf = held.data_ptr()
-        return sf + sf_bytes, sf, sf + sf_bytes + bytes_
+        return sf + sf_bytes, sf, sf + sf_bytes + row_bytes
 
     def _product_mx4(self, unit: int, a, w: Mx4, out, what: str, alpha=1.0, limit=0.0) -> None:
         if w.__class__ is not Mx4 or w.lead or w.gate_up != (unit == 1):
@@ -1620,17 +1626,18 @@ class Ops:
         if ready:
             if a.lead or a.gate_up:
                 raise KernelError(f"{what}: rows are one matrix")
-            codes, scales = a.codes_at, a.scales_at
+            codes, scales, stream = a.codes_at, a.scales_at, self._stream()
         else:
             code, ld, rows = self._mx4_type(a, what), self._mx4_ld(a, k, what), a.data_ptr()
             self._mx4_apart(rows, ((m - 1) * ld + k) * (4 - 2 * code), to, m * n * (4 - 2 * out_type), what)
+            stream = self._stream()
             fused = 0 < few <= 12 and m <= 16 and m * few <= self.MX4_FUSED_TASKS
             if not fused:
-                codes, scales, _ = self._mx4_scratch(m, k, (m + 127) // 128)
+                codes, scales, _ = self._mx4_scratch(stream, m, k, (m + 127) // 128)
                 self.launches += 1
         self.launches += 1
         rc = self._mx4("product")(unit, rows, code, ld, codes, scales, w.codes_at, w.scales_at, to, out_type, m, n, k, few, fused,
-                                  w.settled, alpha, limit, self._status_at, self._stream())
+                                  w.settled, alpha, limit, self._status_at, stream)
         if rc:
             _check(rc, what)
 
@@ -1680,12 +1687,13 @@ class Ops:
         # (many slots: every token is quantised once for all of them; 2,048 tokens x 4,096, six chosen, up: 118 us instead of 129,
         # 400 77 instead of 78.5, but 16 tokens 47 instead of 45)
         once = unit != 0 and top > 1 and slots * -(-k // 256) >= self.MX4_ONCE
-        codes, scales, places = self._mx4_scratch(slots, k, slots // 128 + n_experts + 1, 8 * slots if once else 0)
+        stream = self._stream()
+        codes, scales, places = self._mx4_scratch(stream, slots, k, slots // 128 + n_experts + 1, 8 * slots if once else 0)
         self.launches += (2 if once else 1) - (-n_experts // 1024)
         rc = self._mx4("expert_product")(
             unit, at, code, ld, top, unit != 0, places if once else None, codes, scales, w.codes_at, w.scales_at, to, out_type,
             slots, n_experts, n, k, order.data_ptr(), idx.data_ptr(), offsets.data_ptr(), weight.data_ptr(), scale, alpha,
-            limit, self._status_at, self._stream())
+            limit, self._status_at, stream)
         if rc:
             _check(rc, what)
 

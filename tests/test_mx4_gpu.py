@@ -561,3 +561,46 @@ def test_more_choices_than_lanes(ops, kind):
     """Tokens that are quantised once for 36 slots each."""
     assert 600 * 36 * 2 >= ops.MX4_ONCE
     test_products_by_expert(ops, 600, 40, 2, 36, 300, 48, "even", kind)
+
+
+def test_streams_and_graphs_have_their_own_scratch(ops):
+    """One runtime's products on two streams and out of two graphs, all at once."""
+    g = gen("scratch")
+    w = ops.prepare_weight_mx4((torch.randn(4000, 2100, generator=g) * 0.1).bfloat16().cuda())
+    experts, top, t = 6, 2, 700
+    w1 = ops.prepare_weight_mx4(torch.randn(experts, 2, 200, 2100, generator=g).bfloat16().cuda(), gate_up=True)
+    jobs = []
+    for i in range(4):
+        idx = choices(t, experts, top, "even", g)
+        jobs.append((torch.randn(t, 2100, generator=g).bfloat16().cuda(), torch.empty(t, 4000, device="cuda"),
+                     routed(idx, torch.ones(t, top), experts), torch.empty(t * top, 200, dtype=torch.bfloat16, device="cuda")))
+
+    def run(job):
+        a, out, work, y = job
+        ops.linear_mx4(a, w, out)
+        ops.expert_glu_mx4(a, w1, y, work, top, False)
+
+    want = []
+    for job in jobs:
+        run(job)
+        want.append((job[1].clone(), job[3].clone()))
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for graph, job in zip(graphs, jobs):
+        with torch.cuda.graph(graph):
+            run(job)
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for job in jobs:
+        job[1].fill_(-1.0)
+        job[3].fill_(-1.0)
+    torch.cuda.synchronize()
+    for _ in range(15):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                if i < 2:
+                    graphs[i].replay()
+                else:
+                    run(jobs[i])
+    torch.cuda.synchronize()
+    for job, (out, y) in zip(jobs, want):
+        assert torch.equal(job[1], out) and torch.equal(job[3], y)
+    ops.check_status()
