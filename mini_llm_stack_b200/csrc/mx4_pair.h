@@ -67,11 +67,11 @@ __device__ __forceinline__ void store32(void* at, const uint32_t (&w)[8]) {
                  ::"l"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                  : "memory");
 }
-// COUNT neighbouring outputs of a row, `there` of which exist; vec: the row's runs start at 32-byte places.
+// COUNT neighbouring outputs of a row, `there` of which exist, at a 32-byte place.
 template <typename OUT, int COUNT>
-__device__ __forceinline__ void store_run(OUT* out, const float (&v)[COUNT], int there, bool vec) {
+__device__ __forceinline__ void store_run(OUT* out, const float (&v)[COUNT], int there) {
     constexpr int PER = 32 / sizeof(OUT);
-    if (vec && there >= COUNT) {
+    if (there >= COUNT) {
 #pragma unroll
         for (int i = 0; i < COUNT / PER; ++i) {
             uint32_t w[8];
@@ -90,6 +90,31 @@ __device__ __forceinline__ void store_run(OUT* out, const float (&v)[COUNT], int
 #pragma unroll
         for (int i = 0; i < COUNT; ++i)
             if (i < there) Elem<OUT>::store(out + i, v[i]);
+    }
+}
+
+// 16 neighbouring outputs of the rows of a warp's lanes, at places that suit no wide store: turned within each half of the warp,
+// so that a store takes 16 neighbours of two rows.  (A lane's one by one: 143 us for 2,000 x 14,000 by 3,999 instead of 60.)
+template <typename OUT>
+__device__ __forceinline__ void store_turned(OUT* out, int width, const float (&v)[16], int col, int to, bool mine, int lane) {
+    uint32_t w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[i]);
+#pragma unroll
+    for (int bit = 1; bit < 16; bit *= 2) {
+        const bool upper = lane & bit;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (i & bit) continue;
+            const uint32_t got = __shfl_xor_sync(0xffffffffu, upper ? w[i] : w[i | bit], bit);
+            (upper ? w[i] : w[i | bit]) = got;
+        }
+    }
+    const int n = col + (lane & 15), row = mine ? to : -1;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {                   // the lane's column of row i of its half
+        const int r = __shfl_sync(0xffffffffu, row, (lane & 16) + i);
+        if (r >= 0 && n < width) Elem<OUT>::store(out + (size_t)r * width + n, __uint_as_float(w[i]));
     }
 }
 
@@ -131,7 +156,7 @@ struct To {
 // each to its 32 rows: 152 us instead of 146, at the same sizes).
 template <typename OUT, bool GROUPED, int RUNS, typename Read>
 __device__ __forceinline__ void store_lines(const Product& p, uint32_t d, int set, int sets, bool down, int columns, int n0,
-                                            bool any, const To& to, int lane, bool vec, Read read) {
+                                            bool any, const To& to, int lane, Read read) {
 #pragma unroll 1
     for (int i = 0; i < RUNS; ++i) {
         const int c0 = ((down ? RUNS - 1 - i : i) * sets + set) * 32;
@@ -158,7 +183,7 @@ __device__ __forceinline__ void store_lines(const Product& p, uint32_t d, int se
                 if (GROUPED) v[j] *= to.share[z];
                 if (p.unit == RELU2) v[j] = fmaxf(v[j], 0.f) * fmaxf(v[j], 0.f);
             }
-            if (to.mine[z]) store_run<OUT>((OUT*)p.out + (size_t)to.row[z] * p.width + col, v, p.width - col, vec);
+            if (to.mine[z]) store_run<OUT>((OUT*)p.out + (size_t)to.row[z] * p.width + col, v, p.width - col);
         }
     }
 }
@@ -167,8 +192,8 @@ __device__ __forceinline__ void store_lines(const Product& p, uint32_t d, int se
 // columns apart, in the order in which they are to be read; `read(i)` is called behind the i-th one's reading.
 template <typename OUT, bool GROUPED, int RUNS, typename Read>
 __device__ __forceinline__ void store_rows(const Product& p, uint32_t d, int set, int sets, bool down, int columns, int n0,
-                                           bool any, bool mine, int to, float share, bool vec, Read read) {
-    OUT* row = (OUT*)p.out + (size_t)to * p.width;
+                                           bool any, bool mine, int to, float share, int lane, bool vec, Read read) {
+    OUT *out = (OUT*)p.out, *row = out + (size_t)to * p.width;
     const bool pairs = p.unit == GATED, square = p.unit == RELU2;
 #pragma unroll 1
     for (int i = 0; i < RUNS; ++i) {
@@ -191,17 +216,22 @@ __device__ __forceinline__ void store_rows(const Product& p, uint32_t d, int set
                 v[j] = unit_of_sums<OUT>(g, up, p.alpha, p.limit);
             }
             const int col = (n0 + c0) / 2;
-            if (mine) store_run<OUT>(row + col, v, p.width - col, vec);
+            if (!vec) store_turned<OUT>(out, p.width, v, col, to, mine, lane);
+            else if (mine) store_run<OUT>(row + col, v, p.width - col);
         } else {
-            float v[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-                v[j] = __uint_as_float(j < 16 ? x[j & 15] : y[j & 15]);
-                if (GROUPED) v[j] *= share;
-                if (square) v[j] = fmaxf(v[j], 0.f) * fmaxf(v[j], 0.f);
+            for (int half = 0; half < 2; ++half) {
+                float v[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    v[j] = __uint_as_float(half ? y[j] : x[j]);
+                    if (GROUPED) v[j] *= share;
+                    if (square) v[j] = fmaxf(v[j], 0.f) * fmaxf(v[j], 0.f);
+                }
+                const int col = n0 + c0 + 16 * half;
+                if (!vec) store_turned<OUT>(out, p.width, v, col, to, mine, lane);
+                else if (mine) store_run<OUT>(row + col, v, p.width - col);
             }
-            const int col = n0 + c0;
-            if (mine) store_run<OUT>(row + col, v, p.width - col, vec);
         }
     }
 }
@@ -362,7 +392,7 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
         // Where this thread's rows go and the weights of their slots: numbers of slots read two units ahead, weights one, while
         // instructions run and sums are stored (read when their unit's turn came: 146 us instead of 129 for 2,048 tokens down, six
         // chosen of 64 experts of 4,096 x 1,408)
-        const bool lines = p.unit != GATED && p.out_type != MLS_BF16, look = GROUPED && (p.unit == DOWN || p.scale);
+        const bool lines = p.unit != GATED && p.out_type != MLS_BF16 && vec, look = GROUPED && (p.unit == DOWN || p.scale);
         const int row = (int)rank * UMMA_M + q * 32;               // the warp's first
         auto row_of = [&](int z) { return row + (lines ? lane / 4 + 8 * z : lane); };
         auto unit_at = [&](int i) {
@@ -421,13 +451,13 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
             tc_fence_after();
             const uint32_t at = d + ((uint32_t)(q * 32) << 16);
             if (lines)
-                store_lines<float, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, to, lane, vec, read);
+                store_lines<float, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, to, lane, read);
             else if (p.out_type == MLS_BF16)
                 store_rows<__nv_bfloat16, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, to.mine[0], to.row[0],
-                                                         to.share[0], vec, read);
+                                                         to.share[0], lane, vec, read);
             else
                 store_rows<float, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, to.mine[0], to.row[0],
-                                                 to.share[0], vec, read);
+                                                 to.share[0], lane, vec, read);
             u = u1, u1 = u2, slots = slots1, slots1 = slots2, shares = shares1;
         }
     }
