@@ -25,14 +25,15 @@ struct Tasks {
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-mx4_quantize_kernel(const T* __restrict__ x, long long ld, const Tasks tasks, int K, const RowMap map,
+mx4_quantize_kernel(const T* __restrict__ x, const T* end, long long ld, const Tasks tasks, int K, const RowMap map,
                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     chain_release();
     chain_wait();
     const int pitch = pitch_of(K), atoms = atoms_of(K), lane = threadIdx.x & 31;
     const unsigned first = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     unsigned p = first / tasks.chunks, chunk = first - p * tasks.chunks;
-    Eight<T> held[QUANTIZE_UNROLL][2];
+    Raw<T, VEC, 2> raw[QUANTIZE_UNROLL];
+    const T* from[QUANTIZE_UNROLL];
     unsigned row[QUANTIZE_UNROLL], at[QUANTIZE_UNROLL];
     int slot[QUANTIZE_UNROLL], e[QUANTIZE_UNROLL], o[QUANTIZE_UNROLL];
     // (a slot's number, its expert and that one's first row: loads that wait for one another, but for no other task's)
@@ -53,18 +54,18 @@ mx4_quantize_kernel(const T* __restrict__ x, long long ld, const Tasks tasks, in
     for (int j = 0; j < QUANTIZE_UNROLL; ++j) {
         row[j] = p, at[j] = chunk;
         if (p < tasks.rows) {
-            const unsigned from = map.gather ? (unsigned)(slot[j] / map.top) : p;
-            const int k0 = (int)chunk * QUANTIZE_PART + lane * 16;
-            held[j][0] = load8<T, VEC>(x + (long long)from * ld, k0, K);
-            held[j][1] = load8<T, VEC>(x + (long long)from * ld, k0 + 8, K);
+            from[j] = x + (long long)(map.gather ? (unsigned)(slot[j] / map.top) : p) * ld;
+            load_raw(x, end, from[j], (int)chunk * QUANTIZE_PART + lane * 16, K, raw[j]);
         }
         tasks.next(p, chunk);
     }
 #pragma unroll
     for (int j = 0; j < QUANTIZE_UNROLL; ++j) {
         if (row[j] >= tasks.rows) break;
+        Eight<T> held[2];
+        settle(raw[j], from[j], (int)at[j] * QUANTIZE_PART + lane * 16, K, held);
         uint32_t word, packed[2];
-        quantize_lane(held[j], lane, packed, word);
+        quantize_lane(held, lane, packed, word);
         Place to;
         if (map.offsets) {
             if (e[j] >= map.n_experts) continue;    // a slot of an output without weights: nobody reads it
@@ -102,7 +103,7 @@ mx4_places_kernel(const RowMap map, int slots, int2* __restrict__ places) {
 // codes and scales as rows of their own, copied to the slots by a second kernel: 17).
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
-mx4_tokens_kernel(const T* __restrict__ x, long long ld, const Tasks tasks, int K, int top, int slots, int tiles,
+mx4_tokens_kernel(const T* __restrict__ x, const T* end, long long ld, const Tasks tasks, int K, int top, int slots, int tiles,
                   const int2* __restrict__ places, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     chain_release();
     chain_wait();
@@ -112,12 +113,17 @@ mx4_tokens_kernel(const T* __restrict__ x, long long ld, const Tasks tasks, int 
     for (; token < tasks.rows; tasks.next(token, chunk)) {
         const int k0 = (int)chunk * QUANTIZE_PART + lane * 16;
         const T* row = x + (long long)token * ld;
-        const Eight<T> held[2] = {load8<T, VEC>(row, k0, K), load8<T, VEC>(row, k0 + 8, K)};
+        Raw<T, VEC, 2> raw;
+        load_raw(x, end, row, k0, K, raw);
         const int byte = (int)chunk * (QUANTIZE_PART / 2) + lane * 8, atom = (int)chunk * 4 + (lane >> 3);
         uint32_t word = 0, packed[2];
         for (int j0 = 0; j0 < top; j0 += 32) {
             const int2 mine = j0 + lane < top ? places[(size_t)token * top + j0 + lane] : make_int2(-1, 0);
-            if (j0 == 0) quantize_lane(held, lane, packed, word);
+            if (j0 == 0) {
+                Eight<T> held[2];
+                settle(raw, row, k0, K, held);
+                quantize_lane(held, lane, packed, word);
+            }
             const int n = min(32, top - j0);
             for (int j = 0; j < n; ++j) {
                 const int to = __shfl_sync(0xffffffffu, mine.x, j), at = __shfl_sync(0xffffffffu, mine.y, j);
@@ -135,54 +141,75 @@ mx4_tokens_kernel(const T* __restrict__ x, long long ld, const Tasks tasks, int 
 
 // What codes and scales stand for, in the same tasks.  A lane takes PER neighbouring values, 16 bytes of output, once in 256
 // bfloat16 values and twice in 256 of float32 (two stores of 16 bytes a lane, 32 apart from the next lane's: 62 us for
-// 14,336 x 4,096 instead of 43).
-template <typename T>
+// 14,336 x 4,096 instead of 43).  Without VEC rows begin anywhere.  A lane then stores float32 values one by one; of bfloat16 it takes
+// the values of a 16-byte piece of the output, whose codes may lie in two words and two blocks, and only the pieces at a row's
+// ends are stored so (10,000 x 3,999: 34 us instead of 118).
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256)
 mx4_values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const Tasks tasks, int K,
-                  int rows_per_mat, int pairs, T* __restrict__ out, bool vec) {
+                  int rows_per_mat, int pairs, T* __restrict__ out) {
     chain_release();
     chain_wait();
     constexpr int PER = 16 / sizeof(T), TIMES = 8 / PER;
+    constexpr bool PIECES = !VEC && PER == 8;
     using Word = typename std::conditional<PER == 8, uint32_t, uint16_t>::type;      // PER codes
     const int pitch = pitch_of(K), lane = threadIdx.x & 31;
     const unsigned first = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     unsigned p = first / tasks.chunks, chunk = first - p * tasks.chunks;
-    uint32_t words[UNROLL][TIMES], scale[UNROLL][TIMES];
+    uint32_t words[UNROLL][TIMES], scale[UNROLL][TIMES], scale_behind[UNROLL];
     unsigned row[UNROLL], chunk_of[UNROLL];
+    // a lane's first value in a task (PIECES: of a piece that may begin before the row)
+    auto value = [&](unsigned row, unsigned chunk, int h) {
+        const unsigned before = PIECES ? ((unsigned)(reinterpret_cast<uintptr_t>(out) / sizeof(T)) + row * (unsigned)K) % PER : 0;
+        return (int)(chunk * 256 + (h * 32 + lane) * PER) - (int)before;
+    };
 #pragma unroll
     for (int j = 0; j < UNROLL; ++j) {
         row[j] = p, chunk_of[j] = chunk;
         if (p < tasks.rows) {
             const Place at = place_of(p, rows_per_mat, pairs);
             const uint8_t* row_codes = codes + (size_t)at.row * pitch;
-            const uint8_t* row_scales = scales + ((size_t)at.tile * tasks.chunks + chunk) * (2 * ATOM) + row_in_atom(at.r);
+            if constexpr (PIECES) {
+                const uint8_t* row_scales = scales + (size_t)at.tile * atoms_of(K) * ATOM + row_in_atom(at.r);
+                const int k = value(p, chunk, 0), byte = (k >> 3) * 4;
+                const unsigned k1 = max(k, 0), k2 = min(k + PER - 1, K - 1);
+                uint32_t a = 0, b = 0;
+                if (byte >= 0 && byte < pitch) a = *reinterpret_cast<const uint32_t*>(row_codes + byte);
+                if (byte + 4 < pitch) b = *reinterpret_cast<const uint32_t*>(row_codes + byte + 4);
+                words[j][0] = __funnelshift_r(a, b, 4 * (k & 7));
+                scale[j][0] = k < K ? row_scales[(k1 >> 7) * ATOM + (k1 >> 5 & 3)] : 0;
+                scale_behind[j] = k < K ? row_scales[(k2 >> 7) * ATOM + (k2 >> 5 & 3)] : 0;
+            } else {
+                const uint8_t* task_scales = scales + ((size_t)at.tile * tasks.chunks + chunk) * (2 * ATOM) + row_in_atom(at.r);
 #pragma unroll
-            for (int h = 0; h < TIMES; ++h) {
-                const int k = (h * 32 + lane) * PER, byte = (int)chunk * 128 + k / 2;          // in the task
-                words[j][h] = byte < pitch ? *reinterpret_cast<const Word*>(row_codes + byte) : 0;
-                scale[j][h] = row_scales[k / 128 * ATOM + k / 32 % 4];
+                for (int h = 0; h < TIMES; ++h) {
+                    const int k = (h * 32 + lane) * PER, byte = (int)chunk * 128 + k / 2;          // in the task
+                    words[j][h] = byte < pitch ? *reinterpret_cast<const Word*>(row_codes + byte) : 0;
+                    scale[j][h] = task_scales[k / 128 * ATOM + k / 32 % 4];
+                }
             }
         }
         tasks.next(p, chunk);
     }
+    // (2^(scale - 127); below 2^-126 the power has no exponent field of its own)
+    auto power_of = [](uint32_t c) { return __uint_as_float(c == 255 ? 0x7fffffffu : c ? c << 23 : 0x00400000u); };
 #pragma unroll
     for (int j = 0; j < UNROLL; ++j) {
         if (row[j] >= tasks.rows) break;
 #pragma unroll
         for (int h = 0; h < TIMES; ++h) {
-            const int k0 = (int)chunk_of[j] * 256 + (h * 32 + lane) * PER;
+            const int k0 = value(row[j], chunk_of[j], h);
             if (k0 >= K) continue;
-            // (2^(scale - 127); below 2^-126 the power has no exponent field of its own)
-            const uint32_t c = scale[j][h];
-            const float power = __uint_as_float(c == 255 ? 0x7fffffffu : c ? c << 23 : 0x00400000u);
+            const float power = power_of(scale[j][h]), behind = PIECES ? power_of(scale_behind[j]) : power;
+            const int left = 32 - (k0 & 31);                       // values to the next block
             float v[PER];
 #pragma unroll
             for (int i = 0; i < PER / 2; ++i) {
                 const float2 f = unpack2(words[j][h] >> (8 * i));
-                v[2 * i] = f.x * power, v[2 * i + 1] = f.y * power;
+                v[2 * i] = f.x * (2 * i < left ? power : behind), v[2 * i + 1] = f.y * (2 * i + 1 < left ? power : behind);
             }
             T* dst = out + (size_t)row[j] * K + k0;
-            if (vec) {                               // K is a multiple of PER and the rows are aligned
+            if (VEC || (PIECES && k0 >= 0 && k0 + PER <= K)) {
                 if constexpr (PER == 8) {
                     uint4 w;
                     __nv_bfloat162* b = reinterpret_cast<__nv_bfloat162*>(&w);
@@ -195,7 +222,7 @@ mx4_values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
             } else {
 #pragma unroll
                 for (int i = 0; i < PER; ++i)
-                    if (k0 + i < K) Elem<T>::store(dst + i, v[i]);
+                    if (k0 + i >= 0 && k0 + i < K) Elem<T>::store(dst + i, v[i]);
             }
         }
     }
@@ -222,8 +249,9 @@ int quantize(const void* x, long long ld, long long rows, int K, const RowMap& m
     unsigned blocks;
     if (!tasks_of(rows, K, QUANTIZE_PART, QUANTIZE_UNROLL, tasks, blocks)) return MLS_ERR_UNSUPPORTED;
     auto* kernel = aligned16(x) && ld % (16 / (int)sizeof(T)) == 0 ? mx4_quantize_kernel<T, true> : mx4_quantize_kernel<T, false>;
-    const int rc = chained ? launch_chained(kernel, dim3(blocks), dim3(256), 0, stream, (const T*)x, ld, tasks, K, map, codes, scales)
-                           : launch_plain(kernel, dim3(blocks), dim3(256), 0, stream, (const T*)x, ld, tasks, K, map, codes, scales);
+    const T *first = (const T*)x, *end = first + ((map.gather ? rows / map.top : rows) - 1) * ld + K;
+    const int rc = chained ? launch_chained(kernel, dim3(blocks), dim3(256), 0, stream, first, end, ld, tasks, K, map, codes, scales)
+                           : launch_plain(kernel, dim3(blocks), dim3(256), 0, stream, first, end, ld, tasks, K, map, codes, scales);
     return rc ? rc : launch_status();
 }
 
@@ -234,7 +262,8 @@ int tokens_to_slots(const void* x, long long ld, long long tokens, int K, const 
     unsigned blocks;
     if (!tasks_of(tokens, K, QUANTIZE_PART, 1, tasks, blocks)) return MLS_ERR_UNSUPPORTED;
     auto* kernel = aligned16(x) && ld % (16 / (int)sizeof(T)) == 0 ? mx4_tokens_kernel<T, true> : mx4_tokens_kernel<T, false>;
-    const int rc = launch_plain(kernel, dim3(blocks), dim3(256), 0, stream, (const T*)x, ld, tasks, K, map.top, (int)slots,
+    const T *first = (const T*)x, *end = first + (tokens - 1) * ld + K;
+    const int rc = launch_plain(kernel, dim3(blocks), dim3(256), 0, stream, first, end, ld, tasks, K, map.top, (int)slots,
                                 (int)(slots / TILE_ROWS + map.n_experts + 1), places, codes, scales);
     return rc ? rc : launch_status();
 }
@@ -272,14 +301,21 @@ MLS_API int mls_mx4_values(const void* codes, const void* scales, long long rows
     if (K <= 0 || rows_per_mat <= 0) return MLS_ERR_UNSUPPORTED;
     Tasks tasks;
     unsigned blocks;
-    if (!tasks_of(rows, K, PART_VALUES, UNROLL, tasks, blocks)) return MLS_ERR_UNSUPPORTED;
-    const bool vec = K % (dtype == MLS_BF16 ? 8 : 4) == 0 && aligned16(out);
-    if (dtype == MLS_BF16)
-        MLS_LAUNCH((mx4_values_kernel<__nv_bfloat16>), dim3(blocks), dim3(256), 0, (cudaStream_t)stream,
-                   (const uint8_t*)codes, (const uint8_t*)scales, tasks, K, rows_per_mat, pairs,
-                   (__nv_bfloat16*)out, vec);
-    else
-        MLS_LAUNCH((mx4_values_kernel<float>), dim3(blocks), dim3(256), 0, (cudaStream_t)stream, (const uint8_t*)codes,
-                   (const uint8_t*)scales, tasks, K, rows_per_mat, pairs, (float*)out, vec);
+    const int per = dtype == MLS_BF16 ? 8 : 4;
+    const bool vec = K % per == 0 && aligned16(out);
+    // (bfloat16 rows that begin within a piece of 16 bytes may reach into one more)
+    if (!tasks_of(rows, !vec && per == 8 ? K + per - 1 : K, PART_VALUES, UNROLL, tasks, blocks)) return MLS_ERR_UNSUPPORTED;
+    const cudaStream_t s = (cudaStream_t)stream;
+    const uint8_t *c = (const uint8_t*)codes, *f = (const uint8_t*)scales;
+    const dim3 grid(blocks), block(256);
+    if (dtype == MLS_BF16) {
+        __nv_bfloat16* to = (__nv_bfloat16*)out;
+        if (vec) MLS_LAUNCH((mx4_values_kernel<__nv_bfloat16, true>), grid, block, 0, s, c, f, tasks, K, rows_per_mat, pairs, to);
+        else MLS_LAUNCH((mx4_values_kernel<__nv_bfloat16, false>), grid, block, 0, s, c, f, tasks, K, rows_per_mat, pairs, to);
+    } else {
+        float* to = (float*)out;
+        if (vec) MLS_LAUNCH((mx4_values_kernel<float, true>), grid, block, 0, s, c, f, tasks, K, rows_per_mat, pairs, to);
+        else MLS_LAUNCH((mx4_values_kernel<float, false>), grid, block, 0, s, c, f, tasks, K, rows_per_mat, pairs, to);
+    }
     return launch_status();
 }

@@ -98,33 +98,97 @@ int quantize_rows(const void* x, int dtype, long long ld, long long rows, int K,
 int quantize_tokens(const void* x, int dtype, long long ld, long long tokens, int K, const RowMap& map, long long slots,
                     void* places, uint8_t* codes, uint8_t* scales, cudaStream_t stream);
 
-// Eight neighbouring values of a row as they lie (zeros behind the row's end); VEC: at a 16-byte place.
+// Eight neighbouring values of a row as they lie (zeros behind the row's end).
 template <typename T>
 struct Eight {
     uint32_t w[2 * sizeof(T)];
 };
-template <typename T, bool VEC>
-__device__ __forceinline__ Eight<T> load8(const T* row, int k0, int K) {
-    Eight<T> v;
-    if (VEC && k0 + 8 <= K) {
+// 8 EIGHTS of them as the 16-byte pieces of memory that they lie in, asked for by load_raw and put into place by settle, so that a
+// thread's loads are under way together.  VEC: rows begin at 16-byte places, the values' pieces are theirs alone; else neighbours
+// are read along, of the same matrix (its ends, which may lie within a piece, value by value).
+template <typename T, bool VEC, int EIGHTS>
+struct Raw {
+    static constexpr int OWN = EIGHTS * 8 * sizeof(T) / 16, PIECES = OWN + !VEC;
+    uint4 piece[PIECES];
+};
+template <typename T, bool VEC, int EIGHTS>
+__device__ __forceinline__ void load_raw(const T* matrix, const T* end, const T* row, int k0, int K, Raw<T, VEC, EIGHTS>& r) {
+    if constexpr (VEC) {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
-            const uint4 u = reinterpret_cast<const uint4*>(row + k0)[i];
-            v.w[4 * i] = u.x, v.w[4 * i + 1] = u.y, v.w[4 * i + 2] = u.z, v.w[4 * i + 3] = u.w;
+        for (int e = 0; e < EIGHTS; ++e) {
+            const int k = k0 + 8 * e;
+            uint32_t w[2 * sizeof(T)];
+            if (k + 8 <= K) {
+#pragma unroll
+                for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+                    const uint4 u = reinterpret_cast<const uint4*>(row + k)[i];
+                    w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+                }
+            } else if constexpr (sizeof(T) == 2) {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[i] = (k + 2 * i < K ? (uint32_t)h[k + 2 * i] : 0u) |
+                           (k + 2 * i + 1 < K ? (uint32_t)h[k + 2 * i + 1] << 16 : 0u);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = k + i < K ? __float_as_uint(row[k + i]) : 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+                r.piece[e * (sizeof(T) / 2) + i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
         }
-        return v;
+        return;
     }
-    if constexpr (sizeof(T) == 2) {
-        const uint16_t* h = reinterpret_cast<const uint16_t*>(row);
+    const uintptr_t lo = reinterpret_cast<uintptr_t>(matrix), hi = reinterpret_cast<uintptr_t>(end);
+    const uintptr_t from = reinterpret_cast<uintptr_t>(row + k0) & ~(uintptr_t)15, behind = reinterpret_cast<uintptr_t>(row + K);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            v.w[i] = (k0 + 2 * i < K ? (uint32_t)h[k0 + 2 * i] : 0u) |
-                     (k0 + 2 * i + 1 < K ? (uint32_t)h[k0 + 2 * i + 1] << 16 : 0u);
-    } else {
+    for (int i = 0; i < Raw<T, VEC, EIGHTS>::PIECES; ++i) {
+        const uintptr_t at = from + 16 * i;
+        r.piece[i] = make_uint4(0, 0, 0, 0);
+        if (k0 >= K || at >= behind) continue;
+        if (at >= lo && at + 16 <= hi) {
+            r.piece[i] = *reinterpret_cast<const uint4*>(at);
+        } else {
+            uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v.w[i] = k0 + i < K ? __float_as_uint(row[k0 + i]) : 0u;
+            for (int x = 0; x < 16 / (int)sizeof(T); ++x) {
+                const uintptr_t one = at + x * sizeof(T);
+                if (one < lo || one >= hi) continue;
+                if constexpr (sizeof(T) == 2) w[x / 2] |= (uint32_t)*reinterpret_cast<const uint16_t*>(one) << (x % 2 * 16);
+                else w[x] = *reinterpret_cast<const uint32_t*>(one);
+            }
+            r.piece[i] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
     }
-    return v;
+}
+template <typename T, bool VEC, int EIGHTS>
+__device__ __forceinline__ void settle(const Raw<T, VEC, EIGHTS>& r, const T* row, int k0, int K, Eight<T> (&v)[EIGHTS]) {
+    constexpr int WORDS = 4 * Raw<T, VEC, EIGHTS>::OWN, ALL = 4 * Raw<T, VEC, EIGHTS>::PIECES, PER = 4 / sizeof(T);
+    uint32_t w[ALL];
+#pragma unroll
+    for (int i = 0; i < ALL / 4; ++i)
+        w[4 * i] = r.piece[i].x, w[4 * i + 1] = r.piece[i].y, w[4 * i + 2] = r.piece[i].z, w[4 * i + 3] = r.piece[i].w;
+    if (!VEC) {
+        const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(row + k0) & 15);
+#pragma unroll
+        for (int i = 0; i + 1 < ALL; ++i) w[i] = off & 4 ? w[i + 1] : w[i];
+#pragma unroll
+        for (int i = 0; i + 2 < ALL; ++i) w[i] = off & 8 ? w[i + 2] : w[i];
+        if (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < WORDS; ++i) w[i] = off & 2 ? __funnelshift_r(w[i], w[i + 1], 16) : w[i];
+        }
+    }
+    if (!VEC && k0 + 8 * EIGHTS > K) {
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            if (k0 + i * PER >= K) w[i] = 0;
+            else if (PER == 2 && k0 + i * PER + 1 >= K) w[i] &= 0xffffu;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) v[i / (2 * sizeof(T))].w[i % (2 * sizeof(T))] = w[i];
 }
 
 // Values in [-8, 8] as codes, the first in the lowest bits.

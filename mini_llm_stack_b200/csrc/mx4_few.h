@@ -69,26 +69,27 @@ template <typename T, bool VEC, int NR>
 __device__ __forceinline__ void quantise_slice(const FewProduct& p, int kb0, int n_kb, int worker, int lane, uint8_t* rows) {
     using L = FewPlan<NR, true>;
     // a warp's task: 256 values of a row; warps take them in turn, rows fastest
-    const T* x = (const T*)p.rows + (size_t)kb0 * BK + lane * 8;
-    const int K = p.K - kb0 * BK - lane * 8;
+    const T *x = (const T*)p.rows, *end = x + (p.M - 1) * p.ld + p.K;
     const int step_kb = FEW_WORKERS / p.M, step_r = FEW_WORKERS - step_kb * p.M;
     int kb = worker / p.M, r = worker - kb * p.M;
     constexpr int AT_ONCE = 4;
     while (kb < n_kb) {
-        Eight<T> held[AT_ONCE][1];
+        Raw<T, VEC, 1> raw[AT_ONCE];
         int at_kb[AT_ONCE], at_r[AT_ONCE];
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
             at_kb[j] = kb, at_r[j] = r;
-            if (kb < n_kb) held[j][0] = load8<T, VEC>(x + r * p.ld, kb * BK, K);
+            if (kb < n_kb) load_raw(x, end, x + r * p.ld, (kb0 + kb) * BK + lane * 8, p.K, raw[j]);
             kb += step_kb, r += step_r;
             if (r >= p.M) r -= p.M, ++kb;
         }
 #pragma unroll
         for (int j = 0; j < AT_ONCE; ++j) {
             if (at_kb[j] >= n_kb) break;
+            Eight<T> held[1];
+            settle(raw[j], x + at_r[j] * p.ld, (kb0 + at_kb[j]) * BK + lane * 8, p.K, held);
             uint32_t scales, codes[1];
-            quantize_lane(held[j], lane, codes, scales);
+            quantize_lane(held, lane, codes, scales);
             uint8_t* stage = rows + at_kb[j] * L::ROWS_STAGE;
             // (the 128-byte swizzle: a row's 16-byte pieces change places by the row's number)
             *reinterpret_cast<uint32_t*>(stage + at_r[j] * CODE_ROW + (((lane >> 2) ^ (at_r[j] & 7)) << 4) + (lane & 3) * 4) =

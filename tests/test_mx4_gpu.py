@@ -604,3 +604,72 @@ def test_streams_and_graphs_have_their_own_scratch(ops):
     for job, (out, y) in zip(jobs, want):
         assert torch.equal(job[1], out) and torch.equal(job[3], y)
     ops.check_status()
+
+
+# ------------------------------------------------------------------------------------- rows that suit no wide access
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, k", [(1, 1), (3, 7), (1, 17), (2, 31), (5, 97), (9, 511), (4, 513), (130, 1003), (33, 2049), (700, 333)])
+@pytest.mark.parametrize("before", [0, 1, 3, 6])
+def test_rows_at_any_address(ops, rows, k, dtype, before):
+    """Matrices that begin and end anywhere, among values that are no numbers; back into memory of which nothing else changes."""
+    g = gen("anywhere", rows, k)
+    x = wide_rows(rows, k, g).to(dtype).cuda()
+    ld = k + 2
+    buf = torch.full((before + rows * ld + 40,), float("nan"), dtype=dtype, device="cuda")
+    strided = buf[before:before + rows * ld].view(rows, ld)[:, :k]
+    strided.copy_(x)
+    close = torch.full((before + rows * k + 40,), float("nan"), dtype=dtype, device="cuda")
+    dense = close[before:before + rows * k].view(rows, k)
+    dense.copy_(x)
+    want = torch.empty((rows, k), dtype=torch.float32, device="cuda")
+    ops.mx4_values(ops.quantize_mx4(x.clone()), want)
+    assert same(want.cpu(), plain.nearest(x.cpu()))
+    back = torch.full_like(close, -7.0)
+    for m in (strided, dense):
+        q = ops.quantize_mx4(m)
+        into = back[before:before + rows * k].view(rows, k)
+        into.fill_(-7.0)
+        ops.mx4_values(q, into)
+        assert torch.equal(into.float(), want)
+        assert bool((back[:before] == -7.0).all()) and bool((back[before + rows * k:] == -7.0).all())
+    for m in (1, 5, 16):                                 # and on the way into a product
+        if rows >= m:
+            w = ops.prepare_weight_mx4(torch.randn(40, k, generator=g).cuda())
+            out, same_out = torch.empty(m, 40, device="cuda"), torch.empty(m, 40, device="cuda")
+            ops.linear_mx4(strided[:m], w, out)
+            ops.linear_mx4(x[:m].clone(), w, same_out)
+            assert torch.equal(out, same_out)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("kind", ["plain", "silu", "relu2"])
+@pytest.mark.parametrize("m, n, k", [(700, 1501, 300), (1300, 2047, 520), (515, 3013, 1100), (2050, 777, 64)])
+def test_outputs_that_begin_anywhere(ops, m, n, k, kind, dtype):
+    """Rows of outputs at no 32-byte places, in tiles of many rows; nothing behind them is written."""
+    g = gen("outputs", m, n, k)
+    a = torch.randn(m, k, generator=g).bfloat16()
+    w = (torch.randn(2, n, k, generator=g) * k ** -0.5).bfloat16()
+    buf = torch.full((m * n + 64,), -7.0, dtype=dtype, device="cuda")
+    out = buf[3:3 + m * n].view(m, n)
+    if kind == "silu":
+        ops.linear_glu_mx4(a.cuda(), ops.prepare_weight_mx4(w.cuda(), gate_up=True), out)
+    elif kind == "relu2":
+        ops.linear_relu_squared_mx4(a.cuda(), ops.prepare_weight_mx4(w[0].cuda()), out)
+    else:
+        ops.linear_mx4(a.cuda(), ops.prepare_weight_mx4(w[0].cuda()), out)
+    ops.check_status()
+    assert bool((buf[:3] == -7.0).all()) and bool((buf[3 + m * n:] == -7.0).all())
+    qa, qw = on_device(a.cuda()), on_device(w.cuda())
+    want, off = plain.product(qa, qw[0])
+    if kind == "silu":
+        up, off_up = plain.product(qa, qw[1])
+        want, off = plain.unit(want, up, off, off_up)
+    elif kind == "relu2":
+        z = want.clamp(min=0)
+        want, off = z ** 2, (2 * z + off) * off + z ** 2 * plain.STEPS
+    near(out.cpu(), want.cpu(), off.cpu(), dtype)
+
+
+@pytest.mark.parametrize("kind", ["silu", "relu2"])
+def test_outputs_that_begin_anywhere_by_expert(ops, kind):
+    test_products_by_expert(ops, 1900, 4, 1, 2, 1037, 301, "even", kind)
