@@ -144,8 +144,9 @@ int launch_pair(const Product& p, const void* rows, const void* W, cudaStream_t 
 
 // The ways of many rows, by the tile of a unit of work: 128 weights x 64 or 192 rows on one block, 256 rows x 192 or 256 weights on
 // a pair (routed: 256 x 256 only).  Units are dealt out in rounds of one a block or pair; a round takes so long for every
-// 256 of K, and so long for what its epilogue leaves visible (float32 sums of slots are 200 MB in a long prompt; pairs store them in whole lines).  The
-// cheapest way is taken.  Measured, us, in the order 64 / 192 / 192 on pairs / 256 on pairs, rows quantised already:
+// 256 of K, and so long for what its epilogue leaves visible (float32 sums of slots above all; pairs store them in whole lines).
+// The cheapest way is taken: over 900 products of 17 to 2,048 rows or tokens and 256 to 14,336 of K, 0.5 % behind the fastest on
+// average.  Measured, us, in the order 64 / 192 / 192 on pairs / 256 on pairs, rows quantised already:
 //   256 rows x 14,336, 4,096 outputs       21.4 / 30.3 / 21.5 / 22.5     2,048 rows          125 / 82 / 54 / 42
 //   128 x 4,096, 28,672 gated              23.4 / 16.0 / 20.1 / 17.1     2,048 rows          266 / 134 / 102 / 95
 //   256 x 2,048, 2,048                     5.9 / 10.0 / 8.0 / 8.6        2,048 rows          15.6 / 15.7 / 11.6 / 9.3
@@ -165,12 +166,14 @@ int launch(const Product& p, const void* rows, const void* W, cudaStream_t strea
         return start + (double)((units + places - 1) / places) * (k * per_k + rest);
     };
     const int blocks = sm_count(), pairs = blocks / 2;
-    const double of_192 = 0.30 + 0.00094 * rows_in(192);
-    const double t[4] = {cost(64, 128, blocks, 0.335, 0.45, 0), cost(192, 128, blocks, of_192 > 0.345 ? of_192 : 0.345,
-                                                                     0.9 + 2.5 * slots, 0),
-                         GROUPED ? 1e30 : cost(256, 192, pairs, 0.355, 0.5 + 0.8 * gated, 1),
-                         GROUPED ? cost(256, 256, pairs, 0.30 + 0.0003 * rows_in(256), 0.6 + 0.6 * gated, 1)
-                                 : cost(256, 256, pairs, 0.365, 0.9 + 0.6 * gated, 1)};
+    // (pairs store outputs at odd places row by row)
+    const bool wide = p.width % (p.out_type == MLS_BF16 ? 16 : 8) == 0 && reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
+    const double odd = wide ? 0 : 0.8 + 0.5 * gated;
+    const double t[4] = {cost(64, 128, blocks, 0.325, 0, 0),
+                         cost(192, 128, blocks, 0.263 + 0.001 * rows_in(192), 0.9 + 7.7 * slots, 1.3),
+                         GROUPED ? 1e30 : cost(256, 192, pairs, 0.289, 0.6 + 0.5 * gated + odd, 1.9),
+                         GROUPED ? cost(256, 256, pairs, 0.342, 0.5 + 0.9 * gated, 0.1)
+                                 : cost(256, 256, pairs, 0.24, 0.2 + 1.2 * gated + odd, 4.8)};
     int best = 0;
     for (int way = 1; way < 4; ++way)
         if (t[way] < t[best]) best = way;

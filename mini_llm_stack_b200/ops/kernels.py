@@ -165,7 +165,8 @@ class Mx4:
         all blocks resident at once, two an SM (a block that comes in a second round costs more than its slice saves).
         0: the tiles alone are more, the product takes the way of many rows.  (In us, this way and that one: 8 rows, 4,096
         outputs of 14,336 in eight slices 9.3 and 20.8, 28,672 of 4,096 in one 14.4 and 17.5.  From 17 rows on one or two slices
-        do not pay: 32 rows, 28,672 of 4,096 16.9 and 16.3, 7,168 of 4,096 in four slices 8.4 and 9.3.)"""
+        do not pay: 32 rows, 28,672 of 4,096 16.9 and 16.3, 7,168 of 4,096 in four slices 8.4 and 9.3; nor do from 33 rows on slices of a short K: 45
+        rows, 4,468 of 1,054 8.3 and 6.4, 59 rows, 846 of 2,167 6.9 and 7.6.)"""
         if self._slice is None:
             steps, tiles = -(-self.k // 256), max(1, self.tiles)
             slices = min(8, steps, 2 * sm_count * 19 // 20 // tiles)
@@ -1621,7 +1622,7 @@ class Ops:
         if few is None:
             few = w.few_rows_slice(self.sm_count)
         to = out.data_ptr()
-        if m > 16 and (m > 64 or 4 * few > -(-k // 256)):
+        if m > 16 and (m > 64 or 4 * few > -(-k // 256) or (m > 32 and k <= 7 * 256)):
             few = 0
         if ready:
             if a.lead or a.gate_up:
