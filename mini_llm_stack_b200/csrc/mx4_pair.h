@@ -190,9 +190,9 @@ __device__ __forceinline__ void store_lines(const Product& p, uint32_t d, int se
 
 // A warp's runs of 32 columns of the accumulator, for its 32 rows: this thread's goes to row `to`.  The set's runs lie `step`
 // columns apart, in the order in which they are to be read; `read(i)` is called behind the i-th one's reading.
-template <typename OUT, bool GROUPED, int RUNS, typename Read>
+template <typename OUT, bool GROUPED, int RUNS, bool VEC, typename Read>
 __device__ __forceinline__ void store_rows(const Product& p, uint32_t d, int set, int sets, bool down, int columns, int n0,
-                                           bool any, bool mine, int to, float share, int lane, bool vec, Read read) {
+                                           bool any, bool mine, int to, float share, int lane, Read read) {
     OUT *out = (OUT*)p.out, *row = out + (size_t)to * p.width;
     const bool pairs = p.unit == GATED, square = p.unit == RELU2;
 #pragma unroll 1
@@ -216,7 +216,7 @@ __device__ __forceinline__ void store_rows(const Product& p, uint32_t d, int set
                 v[j] = unit_of_sums<OUT>(g, up, p.alpha, p.limit);
             }
             const int col = (n0 + c0) / 2;
-            if (!vec) store_turned<OUT>(out, p.width, v, col, to, mine, lane);
+            if (!VEC) store_turned<OUT>(out, p.width, v, col, to, mine, lane);
             else if (mine) store_run<OUT>(row + col, v, p.width - col);
         } else {
 #pragma unroll
@@ -229,7 +229,7 @@ __device__ __forceinline__ void store_rows(const Product& p, uint32_t d, int set
                     if (square) v[j] = fmaxf(v[j], 0.f) * fmaxf(v[j], 0.f);
                 }
                 const int col = n0 + c0 + 16 * half;
-                if (!vec) store_turned<OUT>(out, p.width, v, col, to, mine, lane);
+                if (!VEC) store_turned<OUT>(out, p.width, v, col, to, mine, lane);
                 else if (mine) store_run<OUT>(row + col, v, p.width - col);
             }
         }
@@ -452,12 +452,18 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
             const uint32_t at = d + ((uint32_t)(q * 32) << 16);
             if (lines)
                 store_lines<float, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, to, lane, read);
+            else if (vec && p.out_type == MLS_BF16)
+                store_rows<__nv_bfloat16, GROUPED, RUNS, true>(p, at, set, L::SETS, down, columns(u), u.n0, any, to.mine[0],
+                                                               to.row[0], to.share[0], lane, read);
             else if (p.out_type == MLS_BF16)
-                store_rows<__nv_bfloat16, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, to.mine[0], to.row[0],
-                                                         to.share[0], lane, vec, read);
+                store_rows<__nv_bfloat16, GROUPED, RUNS, false>(p, at, set, L::SETS, down, columns(u), u.n0, any, to.mine[0],
+                                                                to.row[0], to.share[0], lane, read);
+            else if (vec)
+                store_rows<float, GROUPED, RUNS, true>(p, at, set, L::SETS, down, columns(u), u.n0, any, to.mine[0], to.row[0],
+                                                       to.share[0], lane, read);
             else
-                store_rows<float, GROUPED, RUNS>(p, at, set, L::SETS, down, columns(u), u.n0, any, to.mine[0], to.row[0],
-                                                 to.share[0], lane, vec, read);
+                store_rows<float, GROUPED, RUNS, false>(p, at, set, L::SETS, down, columns(u), u.n0, any, to.mine[0], to.row[0],
+                                                        to.share[0], lane, read);
             u = u1, u1 = u2, slots = slots1, slots1 = slots2, shares = shares1;
         }
     }
