@@ -57,6 +57,21 @@ static __device__ __forceinline__ float over(float a, float b) {
     const float better = fmaf(fmaf(-q, b, a), r, q);
     return b > 3.402823466e38f || fabsf(q) > 3.402823466e38f ? q : better;      // 0, NaN or infinite already
 }
+// Comparisons that keep what is no number (of a NaN and a number fminf and fmaxf return the number).
+static __device__ __forceinline__ float at_most(float v, float most) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(most));
+    return r;
+}
+static __device__ __forceinline__ float at_least(float v, float least) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(least));
+    return r;
+}
+static __device__ __forceinline__ float relu_squared(float v) {
+    const float r = at_least(v, 0.f);
+    return r * r;
+}
 // a times the logistic function of z.
 static __device__ __forceinline__ float times_sigmoid(float a, float z) { return over(a, 1.0f + expf(-z)); }
 

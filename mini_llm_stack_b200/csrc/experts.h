@@ -11,8 +11,8 @@ constexpr int TC_EXPERTS = 4096;     // experts of a launch: their table lies be
 // The gated unit on the two products' float32 sums.
 __device__ __forceinline__ float gated_unit(float g, float u, float alpha, float limit) {
     if (limit > 0.f) {
-        g = fminf(g, limit);
-        u = fminf(fmaxf(u, -limit), limit);
+        g = at_most(g, limit);
+        u = at_most(at_least(u, -limit), limit);
         return times_sigmoid(g, alpha * g) * (u + 1.0f);
     }
     return times_sigmoid(g, g) * u;

@@ -257,7 +257,7 @@ __device__ __forceinline__ void few_block(const FewProduct& p, const CUtensorMap
             }
             if (pairs) v = p.out_type == MLS_BF16 ? unit_of_sums<__nv_bfloat16>(v, u, p.alpha, p.limit)
                                                   : unit_of_sums<float>(v, u, p.alpha, p.limit);
-            else if (p.unit == RELU2) v = fmaxf(v, 0.f) * fmaxf(v, 0.f);
+            else if (p.unit == RELU2) v = relu_squared(v);
             store_from_float(p.out, (size_t)r * p.width + n, p.out_type, v);
         }
     }

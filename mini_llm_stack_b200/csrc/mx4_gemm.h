@@ -209,8 +209,8 @@ __device__ __forceinline__ float unit_of_sums(float g, float u, float alpha, flo
     if (sizeof(OUT) == 4) return mls_experts::gated_unit(g, u, alpha, limit);
     float z = g;
     if (limit > 0.f) {
-        g = fminf(g, limit);
-        u = fminf(fmaxf(u, -limit), limit) + 1.0f;
+        g = at_most(g, limit);
+        u = at_most(at_least(u, -limit), limit) + 1.0f;
         z = alpha * g;
     }
     float e, r;
@@ -293,7 +293,7 @@ __device__ __forceinline__ void store_unit(const Product& p, const Unit& u, cons
 #pragma unroll
             for (int x = 0; x < 16; ++x, at += p.width) {
                 float val = __uint_as_float(v[x]);
-                if (square) val = fmaxf(val, 0.f) * fmaxf(val, 0.f);
+                if (square) val = relu_squared(val);
                 if (mine && x < there) Elem<OUT>::store(at, val);
             }
         }

@@ -181,7 +181,7 @@ __device__ __forceinline__ void store_lines(const Product& p, uint32_t d, int se
             for (int j = 0; j < 8; ++j) {
                 v[j] = __uint_as_float(w[j / 2][j % 2]);
                 if (GROUPED) v[j] *= to.share[z];
-                if (p.unit == RELU2) v[j] = fmaxf(v[j], 0.f) * fmaxf(v[j], 0.f);
+                if (p.unit == RELU2) v[j] = relu_squared(v[j]);
             }
             if (to.mine[z]) store_run<OUT>((OUT*)p.out + (size_t)to.row[z] * p.width + col, v, p.width - col);
         }
@@ -226,7 +226,7 @@ __device__ __forceinline__ void store_rows(const Product& p, uint32_t d, int set
                 for (int j = 0; j < 16; ++j) {
                     v[j] = __uint_as_float(half ? y[j] : x[j]);
                     if (GROUPED) v[j] *= share;
-                    if (square) v[j] = fmaxf(v[j], 0.f) * fmaxf(v[j], 0.f);
+                    if (square) v[j] = relu_squared(v[j]);
                 }
                 const int col = n0 + c0 + 16 * half;
                 if (!VEC) store_turned<OUT>(out, p.width, v, col, to, mine, lane);
