@@ -371,8 +371,7 @@ expert_gemm_kernel(const T* __restrict__ A, const T* __restrict__ W, void* __res
                 Elem<T>::store((T*)out + (size_t)(p0 + r) * N + n,
                                gated_unit(acc[i][j], acu[i][j], alpha, limit));
             } else if (UP) {
-                const float u = fmaxf(acc[i][j], 0.f);
-                Elem<T>::store((T*)out + (size_t)(p0 + r) * N + n, u * u);
+                Elem<T>::store((T*)out + (size_t)(p0 + r) * N + n, relu_squared(acc[i][j]));
             } else {
                 ((float*)out)[(size_t)slot * N + n] = scale ? acc[i][j] * weight[slot] : acc[i][j];
             }

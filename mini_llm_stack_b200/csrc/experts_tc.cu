@@ -273,7 +273,7 @@ expert_tc_kernel(const TcParams p, const __grid_constant__ CUtensorMap rows_map,
                     } else if (mine && c0 + x < u.rows) {
                         const float r = UNIT == GATED
                                             ? gated_unit(val, __uint_as_float(w[x]), p.alpha, p.limit)
-                                            : fmaxf(val, 0.f) * fmaxf(val, 0.f);
+                                            : relu_squared(val);
                         ((__nv_bfloat16*)p.out)[(size_t)(u.row0 + c0 + x) * p.N + n] =
                             __float2bfloat16_rn(r);
                     }

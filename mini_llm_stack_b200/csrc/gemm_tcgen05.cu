@@ -84,8 +84,8 @@ struct Smem {
 
 __device__ __forceinline__ float gated(float g, float u, float alpha, float limit, float shift) {
     if (limit > 0.f) {
-        g = fminf(g, limit);
-        u = fminf(fmaxf(u, -limit), limit);
+        g = at_most(g, limit);
+        u = at_most(at_least(u, -limit), limit);
     }
     return times_sigmoid(g, alpha * g) * (u + shift);
 }
@@ -104,11 +104,7 @@ __device__ __forceinline__ void gated16(const GemmParams& p, const uint32_t (&g)
 }
 // An activation without a gate on a finished output (epilogue 2: relu(x)^2; else x).
 __device__ __forceinline__ float ungated(int epilogue, float x) {
-    if (epilogue == 2) {
-        x = fmaxf(x, 0.f);
-        return x * x;
-    }
-    return x;
+    return epilogue == 2 ? relu_squared(x) : x;
 }
 
 // Store 16 consecutive columns (col0 ..) of D's row `row`.  With the SwiGLU

@@ -63,8 +63,8 @@ __global__ void swiglu_kernel(const T* __restrict__ gu, T* __restrict__ out, int
 // out = g' * sigmoid(alpha * g') * (u' + 1).  (limit <= 0: no clamping.)
 __device__ __forceinline__ float clamped_glu(float g, float u, float alpha, float limit) {
     if (limit > 0.f) {
-        g = fminf(g, limit);
-        u = fminf(fmaxf(u, -limit), limit);
+        g = at_most(g, limit);
+        u = at_most(at_least(u, -limit), limit);
     }
     return times_sigmoid(g, alpha * g) * (u + 1.0f);
 }
@@ -95,8 +95,7 @@ __global__ void unary_act_kernel(const TI* __restrict__ in, TO* __restrict__ out
          i += (size_t)gridDim.x * blockDim.x) {
         float z = Elem<TI>::load(in + i);
         if (bias) z += load_as_float(bias, i % width, bias_dtype);
-        z = fmaxf(z, 0.f);
-        Elem<TO>::store(out + i, z * z);
+        Elem<TO>::store(out + i, relu_squared(z));
     }
 }
 
