@@ -1513,7 +1513,7 @@ class Ops:
     def _mx4_ld(x, k: int, what: str) -> int:
         """The distance of a matrix's rows, whose values must lie side by side."""
         ld, step = x.stride()
-        if ld >= k and step == 1:
+        if ld >= k and (step == 1 or k == 1):
             return ld
         if (step != 1 and k > 1) or x.shape[0] > 1:
             raise KernelError(f"{what}: a row's values must lie side by side, rows must not overlap")

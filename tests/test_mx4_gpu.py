@@ -673,3 +673,17 @@ def test_outputs_that_begin_anywhere(ops, m, n, k, kind, dtype):
 @pytest.mark.parametrize("kind", ["silu", "relu2"])
 def test_outputs_that_begin_anywhere_by_expert(ops, kind):
     test_products_by_expert(ops, 1900, 4, 1, 2, 1037, 301, "even", kind)
+
+
+def test_one_column(ops):
+    """Matrices [rows, 1] with any stride of their one column."""
+    g = gen("one column")
+    for dtype in (torch.bfloat16, torch.float32):
+        x, w = torch.randn(1, 70, generator=g).to(dtype).cuda().t(), torch.randn(1, 33, generator=g).to(dtype).cuda().t()
+        assert x.stride() == (1, 70)
+        assert same(values(ops, ops.quantize_mx4(x)), plain.nearest(x.cpu()))
+        for m in (70, 5):
+            out = torch.full((m, 33), float("nan"), device="cuda")
+            ops.linear_mx4(x[:m], ops.prepare_weight_mx4(w), out)
+            assert torch.equal(out.cpu().double(), plain.nearest(x[:m].cpu()) @ plain.nearest(w.cpu()).T)   # one exact product each
+    ops.check_status()

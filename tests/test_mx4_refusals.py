@@ -139,3 +139,19 @@ def test_more_experts_than_places_are_numbered_for(ops):
             "offsets": torch.zeros(70001, dtype=torch.int32), "weight": torch.zeros(2)}
     with pytest.raises(KernelError, match="experts"):
         ops.expert_relu_squared_mx4(torch.zeros(1, 1), many, torch.zeros(2, 1), work, 2, False)
+
+
+def test_a_single_column_may_have_any_stride(ops):
+    """[rows, 1] of a transposed row is as contiguous as any: its one column's stride says nothing."""
+    one = torch.zeros(1, 5).t()
+    assert one.is_contiguous() and one.stride() == (1, 5) and one.contiguous().stride() == (1, 5)
+    assert ops._mx4_ld(one, 1, "rows") == 1
+    assert ops._mx4_ld(torch.zeros(7, 30)[:, 4:5], 1, "rows") == 30
+    assert ops._mx4_ld(torch.zeros(1, 30)[:, ::30], 1, "rows") >= 1
+    ops._stream, ops._status_at = lambda: 0, 0
+    for call in (lambda: ops.quantize_mx4(one), lambda: ops.linear_mx4(one, Mx4((3, 1), "cpu"), torch.zeros(5, 3))):
+        with pytest.raises(AssertionError, match="a kernel was asked for"):      # accepted
+            call()
+    for refused in (torch.zeros(1).expand(5, 1), torch.zeros(5, 2).t()[:, :2]):
+        with pytest.raises(KernelError):
+            ops._mx4_ld(refused, refused.shape[1], "rows")
