@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 
 import torch
 
@@ -233,6 +234,7 @@ class Ops:
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._status_at = self.status.data_ptr()
         self._mx4_rows: dict = {}                # quantised rows of the 4-bit products, by stream
+        self._mx4_lock = threading.Lock()        # held from a product's scratch memory to its last launch
         self._attention_libs: dict = {}
         self._attention_lib_handles: dict = {}
         self._split_ctas_per_sm: dict = {}       # head size -> CTAs of the split kernel an SM holds
@@ -1587,7 +1589,7 @@ class Ops:
     def _mx4_scratch(self, stream: int, m: int, k: int, tiles: int, more: int = 0) -> tuple:
         """Addresses of the codes and scales of a product's rows in scratch memory, and of `more` bytes behind them.  Every
         stream has its own, and calls of a captured graph take the graph's: neither other streams' calls nor other graphs
-        write there."""
+        write there; threads that share a stream hold ``_mx4_lock`` until their kernels are launched."""
         sf_bytes, row_bytes = tiles * Mx4.tile_bytes(k), m * Mx4.pitch(k)
         size = sf_bytes + row_bytes + more
         if torch.cuda.is_current_stream_capturing():
@@ -1639,12 +1641,14 @@ class Ops:
             self._mx4_apart(rows, ((m - 1) * ld + k) * (4 - 2 * code), to, m * n * (4 - 2 * out_type), what)
             stream = self._stream()
             fused = 0 < few <= 12 and m <= 16 and m * few <= self.MX4_FUSED_TASKS
-            if not fused:
+        product = self._mx4("product")
+        with self._mx4_lock:
+            if not ready and not fused:
                 codes, scales, _ = self._mx4_scratch(stream, m, k, (m + 127) // 128)
                 self.launches += 1
-        self.launches += 1
-        rc = self._mx4("product")(unit, rows, code, ld, codes, scales, w.codes_at, w.scales_at, to, out_type, m, n, k, few, fused,
-                                  w.settled, alpha, limit, self._status_at, stream)
+            self.launches += 1
+            rc = product(unit, rows, code, ld, codes, scales, w.codes_at, w.scales_at, to, out_type, m, n, k, few, fused, w.settled,
+                         alpha, limit, self._status_at, stream)
         if rc:
             _check(rc, what)
 
@@ -1695,13 +1699,14 @@ class Ops:
         # (many slots: every token is quantised once for all of them; 2,048 tokens x 4,096, six chosen, up: 118 us instead of 129,
         # 400 77 instead of 78.5, but 16 tokens 47 instead of 45)
         once = unit != 0 and top > 1 and slots * -(-k // 256) >= self.MX4_ONCE
-        stream = self._stream()
-        codes, scales, places = self._mx4_scratch(stream, slots, k, slots // 128 + n_experts + 1, 8 * slots if once else 0)
-        self.launches += (2 if once else 1) - (-n_experts // 1024)
-        rc = self._mx4("expert_product")(
-            unit, at, code, ld, top, unit != 0, places if once else None, codes, scales, w.codes_at, w.scales_at, to, out_type,
-            slots, n_experts, n, k, order.data_ptr(), idx.data_ptr(), offsets.data_ptr(), weight.data_ptr(), scale, alpha,
-            limit, self._status_at, stream)
+        stream, product = self._stream(), self._mx4("expert_product")
+        with self._mx4_lock:
+            codes, scales, places = self._mx4_scratch(stream, slots, k, slots // 128 + n_experts + 1, 8 * slots if once else 0)
+            self.launches += (2 if once else 1) - (-n_experts // 1024)
+            rc = product(
+                unit, at, code, ld, top, unit != 0, places if once else None, codes, scales, w.codes_at, w.scales_at, to, out_type,
+                slots, n_experts, n, k, order.data_ptr(), idx.data_ptr(), offsets.data_ptr(), weight.data_ptr(), scale, alpha,
+                limit, self._status_at, stream)
         if rc:
             _check(rc, what)
 

@@ -1,5 +1,6 @@
 """4-bit microscaled rows and their products against 64 bits."""
 
+import threading
 import zlib
 
 import pytest
@@ -687,3 +688,43 @@ def test_one_column(ops):
             ops.linear_mx4(x[:m], ops.prepare_weight_mx4(w), out)
             assert torch.equal(out.cpu().double(), plain.nearest(x[:m].cpu()) @ plain.nearest(w.cpu()).T)   # one exact product each
     ops.check_status()
+
+
+def test_two_threads_on_one_stream(ops):
+    """Products whose rows are quantised in scratch memory of the stream, called by two threads at once; one of them
+    asks for more and more of it."""
+    own = Runtime("cuda:0", torch.bfloat16).ops
+    g = gen("threads")
+    w = own.prepare_weight_mx4((torch.randn(300, 2100, generator=g) * 0.1).bfloat16().cuda())
+    w1 = own.prepare_weight_mx4(torch.randn(4, 72, 2100, generator=g).bfloat16().cuda())
+    jobs = []
+    for sizes in (range(70, 1500, 130), range(1400, 60, -130)):
+        calls = []
+        for m in sizes:
+            a = torch.randn(m, 2100, generator=g).bfloat16().cuda()
+            work = routed(choices(m, 4, 1, "even", g), torch.ones(m, 1), 4)
+            calls.append((a, work, torch.empty(m, 300, device="cuda"), torch.empty(m, 72, device="cuda")))
+        jobs.append(calls)
+
+    def run(calls):
+        for a, work, out, y in calls:
+            own.linear_mx4(a, w, out)
+            own.expert_relu_squared_mx4(a, w1, y, work, 1, False)
+
+    for calls in jobs:
+        run(calls)
+    want = [[(out.clone(), y.clone()) for _, _, out, y in calls] for calls in jobs]
+    for _, _, out, y in sum(jobs, []):
+        out.fill_(-1.0)
+        y.fill_(-1.0)
+    own._mx4_rows.clear()
+    threads = [threading.Thread(target=lambda c=calls: [run(c) for _ in range(5)]) for calls in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for calls, results in zip(jobs, want):
+        for (_, _, out, y), (out_want, y_want) in zip(calls, results):
+            assert torch.equal(out, out_want) and torch.equal(y, y_want)
+    own.check_status()

@@ -2,6 +2,8 @@
 
 import copy
 import pickle
+import threading
+import time
 
 import pytest
 import torch
@@ -155,3 +157,39 @@ def test_a_single_column_may_have_any_stride(ops):
     for refused in (torch.zeros(1).expand(5, 1), torch.zeros(5, 2).t()[:, :2]):
         with pytest.raises(KernelError):
             ops._mx4_ld(refused, refused.shape[1], "rows")
+
+
+@pytest.mark.parametrize("routed", [False, True])
+def test_calls_of_two_threads_do_not_come_between_one_another(ops, monkeypatch, routed):
+    """Quantisation and product are two kernels of a call that runs without the interpreter's lock, with scratch memory of
+    the stream between them: a second thread's call on that stream waits for both, and for a larger buffer in the first one's place."""
+    ops._stream, ops._status_at, ops._mx4_rows, ops._mx4_lock = lambda: 0, 0, {}, threading.Lock()
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    inside, met = [], []
+
+    def kernels(*args):
+        inside.append(threading.get_ident())
+        held = ops._mx4_rows[0].data_ptr()
+        time.sleep(0.002)
+        met.append(len(inside) == 1 and ops._mx4_rows[0].data_ptr() == held)
+        inside.pop()
+        return 0
+
+    ops._part_libs = {"mx4": {"product": kernels, "expert_product": kernels}}
+    w, experts = Mx4((40, 4096), "cpu"), Mx4((2, 40, 4096), "cpu")
+
+    def calls(sizes):
+        for m in sizes:
+            if routed:
+                work = {n: torch.zeros(m + 3, dtype=torch.int32) for n in ("order", "idx", "offsets")}
+                ops.expert_relu_squared_mx4(torch.zeros(m, 4096), experts, torch.zeros(m, 40),
+                                            dict(work, weight=torch.zeros(m)), 1, False)
+            else:
+                ops.linear_mx4(torch.zeros(m, 4096), w, torch.zeros(m, 40))
+
+    threads = [threading.Thread(target=calls, args=(range(m, m + 2000, 199),)) for m in (100, 150)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(met) == 22 and all(met)
