@@ -37,10 +37,10 @@ class EngineOptions:
     dtype: str | None = None          # None: the model folder's own dtype
     device: str = "cuda:0"
     kv_dtype: str | None = None       # type of the cached keys and values; None: the run's dtype
-    ffn_weights: str | None = None    # how feed-forward weights are held; "mxfp4": 4-bit microscaled values; None: as loaded
     seed: int = 0                     # sampling seed of requests that bring none
     cuda_graphs: bool = True          # replay decode steps (and repeated, host-bound prompt steps) from graphs
     launch_ahead: bool = True         # start the next decode step before the host has this one's tokens
+    ffn_weights: str | None = None    # how feed-forward weights are held; "mxfp4": 4-bit microscaled values; None: as loaded
 
     def __post_init__(self):
         for k in ("num_blocks", "block_size", "max_batch", "max_tokens_per_step",

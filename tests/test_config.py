@@ -168,3 +168,11 @@ def test_engine_options_refuse_what_contradicts_the_loaded_model():
         EngineOptions(dtype="float32", device="cpu").check_against("bfloat16", "cpu")
     with pytest.raises(ConfigError, match="device"):
         EngineOptions(device="cuda:1").check_against("bfloat16", "cuda:0")
+
+
+def test_engine_options_by_place():
+    """Options may be given in order: new ones come behind those that were there."""
+    from mini_llm_stack_b200.config import EngineOptions
+    opts = EngineOptions(64, 16, 4, 256, 128, "bf16", "cpu", "bfloat16", 7, False, False)
+    assert opts.kv_dtype == "bfloat16" and opts.seed == 7 and not opts.cuda_graphs and not opts.launch_ahead
+    assert opts.ffn_weights is None
