@@ -18,8 +18,12 @@
 //
 // Hand-overs inside the pair, as in the bfloat16 product: full[s] (first block) counts both blocks' copies; empty[s] and acc_full[a]
 // arrive on both blocks' barriers; acc_free[a] and acc_empty[a] (first block) take the arrivals of both blocks' epilogue warps,
-// when they have read the half of an accumulator that the next may take, and all of it.  No load is multicast.  These kernels are launched
-// plainly: chained behind a long quantisation of rows a run under a profiler did not end.
+// when they have read the half of an accumulator that the next may take, and all of it.  No load is multicast.
+//
+// These kernels are launched plainly.  Chained behind a quantisation whose blocks came in several rounds and let their successors start
+// at once, a run under a profiler did not end; what it waited for, reading did not show.  (Without a bound are the allocation of
+// tensor memory, the wait for the kernels in front and the cluster's barriers, and at those every thread arrives whatever ran out
+// before.)  Nothing stands in that place any more: such a quantisation lets nobody start early (mx4.cu, `at_once`).
 //
 // What bounds it: operands out of L2 (2,048 x 14,336 by 4,096 in 44 us, 5.5 PFLOP/s; 2,048 tokens, six of 64 experts, gate and up
 // 2 x 1,408 of 4,096 in 100 us, 70 without copies), and where float32 sums of slots are stored, memory (down 1,408 by 4,096 in 84 us

@@ -63,3 +63,13 @@ def test_every_wait_is_bounded():
         text = re.sub(r"//[^\n]*", "", p.read_text())
         assert not re.search(r"while \(!?\s*mbar_|for \(;;\)|__nanosleep", text), p.name
         assert "multicast::cluster" not in text, p.name
+
+
+def test_long_quantisations_release_nobody_early():
+    """A kernel whose blocks come one after another lets its successors start only at its end: those with tensor memory and
+    clusters would else hold SMs while blocks in front of them still come and go."""
+    text = re.sub(r"//[^\n]*", "", (CSRC / "mx4.cu").read_text())
+    releases = re.findall(r"[^;{}]*chain_release\(\);", text)
+    assert len(releases) == 2 and all("if (tasks.at_once)" in r for r in releases)
+    assert re.search(r"const unsigned room = 4u \* \(unsigned\)sm_count\(\)", text)
+    assert re.search(r"tasks = \{[^;]*blocks <= room\};", text)
