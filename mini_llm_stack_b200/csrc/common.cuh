@@ -228,7 +228,8 @@ static inline int launch_status() { return (int)cudaGetLastError(); }
 // of that kernel's results, and everything it writes, comes after `chain_wait`,
 // which returns once all earlier kernels have finished and their writes are
 // visible.  Between the two a kernel may only touch memory that no kernel writes
-// (weights).  Both are no-ops in a kernel that was launched the plain way.
+// (weights).  In a kernel that was launched the plain way `chain_wait` returns at once;
+// its `chain_release` lets a chained successor start early all the same.
 // A kernel with tensor memory releases its successors from the warp that allocates, once it has
 // allocated: a successor that is resident earlier could take columns that a block here still waits
 // for, and itself wait for this kernel's end.  One thread's call counts for its block.

@@ -202,8 +202,10 @@ __device__ __forceinline__ void row_tiles(const Product& p, int lane, int* start
 }
 
 // The gated unit on two sums on its way to 16 bits: exponential and reciprocal by the approximations of the special function
-// unit, whose 2^-21 or so vanish in the rounding to 2^-8 (in float32's precision, and by half as many warps, the unit kept a product
-// of 2,048 x 2,048 with 16,384 gated sums waiting: 55 us instead of 40).  Outputs of 32 bits take the precise one.
+// unit.  Relative to the output they are off by about 2^-21 around zero; the exponent's rounding makes that grow with |z|, to
+// about 2^-18 where the exponential ends (|z| = 88), a thousandth of the rounding to 2^-8.  (In float32's precision, and by half as
+// many warps, the unit kept a product of 2,048 x 2,048 with 16,384 gated sums waiting: 55 us instead of 40.)  Outputs of 32 bits take
+// the precise one.
 template <typename OUT>
 __device__ __forceinline__ float unit_of_sums(float g, float u, float alpha, float limit) {
     if (sizeof(OUT) == 4) return mls_experts::gated_unit(g, u, alpha, limit);

@@ -386,8 +386,11 @@ __device__ __forceinline__ void pair_block(const Product& p, const CUtensorMap* 
         // two runs of 32 columns a set: the first of 256 in the columns that the next accumulator may take
         constexpr int RUNS = L::NT / 32 / L::SETS, FREE_AT = L::NT == 256 ? RUNS / 2 - 1 : RUNS - 1;
         const bool vec = p.width % (p.out_type == MLS_BF16 ? 16 : 8) == 0 && reinterpret_cast<uintptr_t>(p.out) % 32 == 0;
-        // (relaxed: the fence orders what was read from tensor memory; a release waits for the stores of the runs before as
-        // well, 22.5 us instead of 18.9 for 707 rows x 2,048 by 16,384 gated sums)
+        // Relaxed is enough: what is handed over are columns of tensor memory, nothing in ordinary memory.  PTX orders tensor-memory
+        // operations of different threads by wait::ld (of the whole warp, as the load: lane 0's are the warp's),
+        // fence::before_thread_sync and an arrival on one side, a wait for it and fence::after_thread_sync on the other, and gives
+        // that pattern with relaxed arrivals of the cluster's scope; the wait here even acquires.  A release would wait for the
+        // stores of the runs before as well: 22.5 us instead of 18.9 for 707 rows x 2,048 by 16,384 gated sums.
         auto arrive = [&](uint32_t bar) {
             tc_fence_before();
             __syncwarp();

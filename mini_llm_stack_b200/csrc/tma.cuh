@@ -117,7 +117,8 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar, uint32_t cta) {
         ::"r"(bar), "r"(cta) : "memory");
 }
 // The same without ordering of this thread's own memory operations: for passing on the
-// completion of copies made by the TMA unit, which the waiting barrier has already seen.
+// completion of copies made by the TMA unit, which a barrier has already seen, or of loads
+// from tensor memory (behind wait::ld and fence::before_thread_sync, which order those).
 __device__ __forceinline__ void mbar_arrive_remote_relaxed(uint32_t bar, uint32_t cta) {
     asm volatile(
         "{\n\t.reg .b32 r;\n\t"

@@ -1484,7 +1484,10 @@ class Ops:
     MX4_MOST_ROWS = 1 << 28  # rows of a matrix, and of a weight's matrices together
     MX4_MOST_EXPERTS = 1 << 16
     MX4_ONCE = 1 << 15       # slots x steps of 256 of K from which on tokens are quantised once
-    MX4_FUSED_TASKS = 64     # 256 values of a row each: with so many a block the product quantises its rows itself
+    # 256 values of a row each: with so many a block the product quantises its rows itself.  Us, in the product and in front of it, in
+    # a graph: 32 tasks (8 rows, 4,096 outputs of 8,192) 6.8 and 7.0, 64 (16 rows) 8.7 and 7.2, 112 (16 of 14,336) 12.1 and 9.4;
+    # called from the host, a launch fewer: 7.4 and 11.3, 8.8 and 11.3, 12.4 and 11.3
+    MX4_FUSED_TASKS = 64
 
     def _mx4(self, name: str):
         fns = self._part_libs.get("mx4")
