@@ -728,3 +728,25 @@ def test_two_threads_on_one_stream(ops):
         for (_, _, out, y), (out_want, y_want) in zip(calls, results):
             assert torch.equal(out, out_want) and torch.equal(y, y_want)
     own.check_status()
+
+
+@pytest.mark.parametrize("m", [1, 12, 60, 300])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_longest_rows(ops, m, dtype):
+    """K as long as it may be, from its first value to its last."""
+    n, k = 130, ops.MX4_MOST_K
+    g = torch.Generator("cuda").manual_seed(m)
+    a = torch.randn(m, k, generator=g, device="cuda").to(dtype)
+    w = (torch.randn(n, k, generator=g, device="cuda") * k ** -0.5).bfloat16()
+    q = ops.quantize_mx4(a)
+    back = torch.empty_like(a)
+    ops.mx4_values(q, back)
+    assert torch.equal(back.double(), on_device(a))
+    held = ops.prepare_weight_mx4(w)
+    want, off = plain.product(on_device(a), on_device(w))
+    for rows in (a, q):
+        out = torch.full((m, n), float("nan"), device="cuda")
+        ops.linear_mx4(rows, held, out)
+        ops.check_status()
+        far = (out.double() - want).abs() - off - plain.rounding(torch.float32, want)
+        assert bool((far <= 0).all()), float(far.max())
