@@ -17,10 +17,9 @@ constexpr int UNROLL = 4, PART_VALUES = 256;                       // of values 
 constexpr int QUANTIZE_UNROLL = 2, QUANTIZE_PART = 512;           // of values quantised
 struct Tasks {
     unsigned rows, chunks, step_row, step_chunk;
-    // All blocks are resident at once.  Only then does a kernel let its successors start early: a successor with tensor memory, a
-    // whole SM a block and blocks that wait for one another must not come while blocks in front of it are still exchanged
-    // (a pair's product behind a quantisation of many rounds of blocks did not end under a profiler, for a reason that reading
-    // did not show).  It costs nothing: 14,336 x 4,096 float32 values there and back in 87.3 us, 88.1 with early starts.
+    // All blocks are resident at once.  Only then does a kernel let its successors start early: one with tensor memory, a whole SM a
+    // block and blocks that wait for one another shall not become resident SM by SM while the last round of many drains (a
+    // pair's product behind such a quantisation did not end under a profiler, for a reason that reading did not show).  It costs nothing: 14,336 x 4,096 float32 values there and back in 87.3 us, 88.1 with early starts.
     bool at_once;
     __device__ __forceinline__ void next(unsigned& row, unsigned& chunk) const {
         row += step_row, chunk += step_chunk;

@@ -186,8 +186,8 @@ int launch(const Product& p, const void* rows, const void* W, cudaStream_t strea
     return launch_pair<256, GROUPED>(p, rows, W, stream);
 }
 
-// Chained, behind a quantisation too: blocks that hold tensor memory and wait for their cluster come only when every block of the
-// kernel in front is resident or has ended, as quantisations of more blocks than that let nobody start early (mx4.cu).
+// Chained, behind a quantisation too: one of a single round of blocks.  Longer ones let nobody start early (mx4.cu), so that no block that
+// holds tensor memory and waits for its cluster becomes resident while they drain.
 template <int NR, bool FUSED>
 int launch_few(const FewProduct& p, const void* rows, const void* W, cudaStream_t stream) {
     using L = FewPlan<NR, FUSED>;

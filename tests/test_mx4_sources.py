@@ -66,8 +66,8 @@ def test_every_wait_is_bounded():
 
 
 def test_long_quantisations_release_nobody_early():
-    """A kernel whose blocks come one after another lets its successors start only at its end: those with tensor memory and
-    clusters would else hold SMs while blocks in front of them still come and go."""
+    """A kernel whose blocks come in several rounds lets its successors start only at its end: those with tensor memory and
+    clusters would else take SMs one by one while its last round drains."""
     text = re.sub(r"//[^\n]*", "", (CSRC / "mx4.cu").read_text())
     releases = re.findall(r"[^;{}]*chain_release\(\);", text)
     assert len(releases) == 2 and all("if (tasks.at_once)" in r for r in releases)
