@@ -15,11 +15,13 @@ using namespace mls_mx4;
 // are warps, whose loads are under way together.
 constexpr int UNROLL = 4, PART_VALUES = 256;                       // of values read back
 constexpr int QUANTIZE_UNROLL = 2, QUANTIZE_PART = 512;           // of values quantised
+constexpr int RESIDENT = 3;                                       // blocks that fit an SM, at least
 struct Tasks {
     unsigned rows, chunks, step_row, step_chunk;
-    // All blocks are resident at once.  Only then does a kernel let its successors start early: one with tensor memory, a whole SM a
-    // block and blocks that wait for one another shall not become resident SM by SM while the last round of many drains (a
-    // pair's product behind such a quantisation did not end under a profiler, for a reason that reading did not show).  It costs nothing: 14,336 x 4,096 float32 values there and back in 87.3 us, 88.1 with early starts.
+    // All blocks are resident at once (RESIDENT an SM).  Only then does a kernel let its successors start early: one with tensor
+    // memory, a whole SM a block and blocks that wait for one another shall not become resident SM by SM while the last round of
+    // many drains (a pair's product behind such a quantisation did not end under a profiler, for a reason that reading did not
+    // show).  It costs nothing: 14,336 x 4,096 float32 values there and back in 87.3 us, 88.1 with early starts.
     bool at_once;
     __device__ __forceinline__ void next(unsigned& row, unsigned& chunk) const {
         row += step_row, chunk += step_chunk;
@@ -28,7 +30,7 @@ struct Tasks {
 };
 
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, RESIDENT)
 mx4_quantize_kernel(const T* __restrict__ x, const T* end, long long ld, const Tasks tasks, int K, const RowMap map,
                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     if (tasks.at_once) chain_release();
@@ -145,7 +147,7 @@ mx4_tokens_kernel(const T* __restrict__ x, const T* end, long long ld, const Tas
 // the values of a 16-byte piece of the output, whose codes may lie in two words and two blocks, and only the pieces at a row's
 // ends are stored so (10,000 x 3,999: 34 us instead of 118).
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2 * RESIDENT)
 mx4_values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, const Tasks tasks, int K,
                   int rows_per_mat, int pairs, T* __restrict__ out) {
     if (tasks.at_once) chain_release();
@@ -238,7 +240,8 @@ bool tasks_of(long long rows, int K, int part, int unroll, Tasks& tasks, unsigne
     const unsigned room = 4u * (unsigned)sm_count(), each = (unsigned)((n + 7) / 8);
     if (blocks < room) blocks = each < room ? each : room;
     const unsigned warps = 8 * blocks;
-    tasks = {(unsigned)rows, (unsigned)chunks, warps / (unsigned)chunks, warps % (unsigned)chunks, blocks <= room};
+    tasks = {(unsigned)rows, (unsigned)chunks, warps / (unsigned)chunks, warps % (unsigned)chunks,
+             blocks <= RESIDENT * (unsigned)sm_count()};
     return true;
 }
 

@@ -71,5 +71,5 @@ def test_long_quantisations_release_nobody_early():
     text = re.sub(r"//[^\n]*", "", (CSRC / "mx4.cu").read_text())
     releases = re.findall(r"[^;{}]*chain_release\(\);", text)
     assert len(releases) == 2 and all("if (tasks.at_once)" in r for r in releases)
-    assert re.search(r"const unsigned room = 4u \* \(unsigned\)sm_count\(\)", text)
-    assert re.search(r"tasks = \{[^;]*blocks <= room\};", text)
+    assert len(re.findall(r"__launch_bounds__\(256, (?:2 \* )?RESIDENT\)\s*mx4_(?:quantize|values)_kernel", text)) == 2
+    assert re.search(r"tasks = \{[^;]*blocks <= RESIDENT \* \(unsigned\)sm_count\(\)\};", text)
