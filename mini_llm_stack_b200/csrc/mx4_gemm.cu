@@ -95,8 +95,8 @@ bool scales_map(const void* ptr, long long tiles, int K, int box_tiles, CUtensor
 
 // Products of many rows are long: their kernels start when the ones before have finished, as those of a step of many tokens
 // do (common.cuh).  Those of fewer rows are chained if all blocks that quantise them are resident at once.  Us, chained and not: 65 rows
-// x 4,096, 4,096 outputs 9.8 and 10.9, 256 rows 10.8 and 11.6, 84 x 14,336 22.5 and 23.9; beyond the rule 200 x 14,336 23.4 and 24.1,
-// 400 x 4,096 12.7 both, 700 x 2,048, 2,048 outputs 9.9 and 10.0, 1,500 rows 11.4 and 10.9.
+// x 4,096, 4,096 outputs 9.1 and 9.9, 256 rows 10.1 and 10.5, 84 x 14,336 21.9 and 23.2; beyond the rule 200 x 14,336 23.4 and 24.2,
+// 400 x 4,096 12.7 and 13.0, 700 x 2,048, 2,048 outputs 9.9 both, 1,500 rows 11.4 and 10.7.
 bool chained(long long rows, int K) { return rows <= 256 && rows * ((K + 255) / 256) <= 32LL * sm_count(); }
 
 template <int NT, bool GROUPED>
